@@ -13,7 +13,7 @@ import os
 from .build import LIB_PATH
 
 OK, EINVAL, EALIGN, ECUDA, ETIMEOUT, EUNSUPPORTED = 0, 1, 2, 3, 4, 5
-F16, F32, I8 = 0, 1, 2
+F16, F32, I8, E4M3 = 0, 1, 2, 3
 ACT_NONE, ACT_GELU = 0, 1
 
 _ERR_NAMES = {
@@ -46,6 +46,10 @@ PROTOTYPES = {
     "dtas_gemv_fused": (_i, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i, _i, _i, _i, _p]),
     "dtas_gemm_nt_static_scratch": (_i, [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i, _i, _i, _p, _p]),
     "dtas_gemm_nt_static_scratch_plan": (_i, [_i64, _i64, _i64, _i, ctypes.POINTER(_i), ctypes.POINTER(_i)]),
+    "dtas_add_rms_norm": (_i, [_p, _p, _p, _p, _p, _p, _i64, _i64, _f, _i, _i, _i, _p]),
+    "dtas_quantize": (_i, [_p, _p, _p, _i64, _i64, _i, _i, _i, _p]),
+    "dtas_gemv_w4": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i, _i, _i, _i, _p]),
+    "dtas_gemm_nt_f8": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i, _i, _i, _p]),
     "dtas_bucket_of": (_i, [ctypes.c_char_p, _i64]),
     "dtas_bucket_count": (_i, [ctypes.c_char_p]),
     "dtas_variant_of": (_i, [ctypes.c_char_p, _i64, _i64, _i64, _i, ctypes.c_char_p, _i]),

@@ -141,7 +141,7 @@ inline int dtype_size(int dt) {
   switch (dt) {
     case DTAS_F16: return 2;
     case DTAS_F32: return 4;
-    case DTAS_I8: return 1;
+    case DTAS_I8: case DTAS_E4M3: return 1;
     default: return 0;
   }
 }
@@ -167,14 +167,27 @@ int launch_row_op(RowOp op, const void* x, const void* p0, const void* p1, void*
 void row_variant_name(RowOp op, int64_t m, int64_t n_cols, char* buf, int len);
 void row_set_override(int tpr);
 
+int launch_add_rms_norm(const void* x, const void* res, const void* weight, void* y, void* res_out, float* scale,
+                        int64_t m, int64_t n_cols, float eps, int in_dtype, int out_dtype, cudaStream_t st);
+int launch_quantize(const void* x, void* q, float* scale, int64_t m, int64_t n_cols, int in_dtype, int out_dtype,
+                    cudaStream_t st);
+void gemv_w4_variant_name(int64_t m, int64_t n, int64_t k, char* buf, int len);
+void row_quant_variant_name(const char* op, int64_t m, int64_t n_cols, char* buf, int len);
+
+int launch_gemv_w4(const void* x, const float* x_scale, const void* w, const void* w_scale, const void* w_zero,
+                   const Epilogue& epi, void* y, int64_t m, int64_t n, int64_t k, int64_t group, int x_dtype,
+                   cudaStream_t st);
+
 int launch_gemv(const void* x, const void* w, const Epilogue& epi, void* y, int64_t n, int64_t k,
                 const DeviceCtx* ctx, cudaStream_t st);
 void gemv_variant_name(int64_t n, int64_t k, const DeviceCtx* ctx, char* buf, int len);
 void gemv_set_override(int wpr, int unroll);
 
 int launch_gemm(const void* x, const void* w, const Epilogue& epi, void* y, int64_t m, int64_t n,
-                int64_t k, int64_t ldy, DeviceCtx* ctx, cudaStream_t st, const PeerOut* peers = nullptr);
+                int64_t k, int64_t ldy, DeviceCtx* ctx, cudaStream_t st, const PeerOut* peers = nullptr,
+                bool f8 = false);   // f8: x and w are e4m3, scaled by epi.sx / epi.sw
 void gemm_variant_name(int64_t m, int64_t n, int64_t k, const DeviceCtx* ctx, char* buf, int len);
+void gemm_f8_variant_name(int64_t m, int64_t n, int64_t k, const DeviceCtx* ctx, char* buf, int len);
 void gemm_set_override(int bn, int split_k);
 int gemm_table_set(int64_t n, int64_t k, int64_t m_lo, int64_t m_hi, int bn, int split_k);
 void gemm_table_clear();

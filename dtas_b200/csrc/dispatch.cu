@@ -90,9 +90,10 @@ int check_rows_cols(const char* op, int64_t m, int64_t n_cols) {
 }
 
 int op_index(const char* op) {
-  static const char* names[] = {"cast", "add", "copy", "rms_norm", "softmax", "layer_norm", "gemv", "gemm"};
+  static const char* names[] = {"cast", "add", "copy", "rms_norm", "softmax", "layer_norm", "gemv", "gemm",
+                                "add_rms_norm", "quantize", "gemv_w4", "gemm_f8"};
   if (op == nullptr) return -1;
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < (int)(sizeof(names) / sizeof(names[0])); ++i)
     if (strcmp(op, names[i]) == 0) return i;
   return -1;
 }
@@ -295,6 +296,104 @@ int dtas_gemm_nt_fused(const void* x, const void* w, const void* bias, const voi
   return launch_add_residuals(y, res1, res2, m * n, c.ctx, c.stream, bucket_of(m));
 }
 
+int dtas_add_rms_norm(const void* x, const void* res, const void* weight, void* y, void* res_out, float* scale,
+                      int64_t m, int64_t n_cols, float eps, int in_dtype, int out_dtype, int device, void* stream) {
+  DTAS_NONNULL("add_rms_norm", x);
+  DTAS_NONNULL("add_rms_norm", weight);
+  DTAS_NONNULL("add_rms_norm", y);
+  int rc = check_rows_cols("add_rms_norm", m, n_cols);
+  if (rc) return rc;
+  if (in_dtype != DTAS_F16 && in_dtype != DTAS_F32)
+    DTAS_FAIL(DTAS_EUNSUPPORTED, "add_rms_norm: the input is fp16 or fp32 (dtype %d)", in_dtype);
+  if (out_dtype != DTAS_F16 && out_dtype != DTAS_I8 && out_dtype != DTAS_E4M3)
+    DTAS_FAIL(DTAS_EUNSUPPORTED, "add_rms_norm: the output is fp16, int8 or e4m3 (dtype %d)", out_dtype);
+  if (out_dtype != DTAS_F16) DTAS_NONNULL("add_rms_norm", scale);
+  Call c;
+  if ((rc = c.begin(device, stream))) return rc;
+  return launch_add_rms_norm(x, res, weight, y, res_out, scale, m, n_cols, eps, in_dtype, out_dtype, c.stream);
+}
+
+int dtas_quantize(const void* x, void* q, float* scale, int64_t m, int64_t n_cols, int in_dtype, int out_dtype,
+                  int device, void* stream) {
+  DTAS_NONNULL("quantize", x);
+  DTAS_NONNULL("quantize", q);
+  DTAS_NONNULL("quantize", scale);
+  int rc = check_rows_cols("quantize", m, n_cols);
+  if (rc) return rc;
+  if (in_dtype != DTAS_F16 && in_dtype != DTAS_F32)
+    DTAS_FAIL(DTAS_EUNSUPPORTED, "quantize: the input is fp16 or fp32 (dtype %d)", in_dtype);
+  if (out_dtype != DTAS_I8 && out_dtype != DTAS_E4M3)
+    DTAS_FAIL(DTAS_EUNSUPPORTED, "quantize: the output is int8 or e4m3 (dtype %d)", out_dtype);
+  Call c;
+  if ((rc = c.begin(device, stream))) return rc;
+  return launch_quantize(x, q, scale, m, n_cols, in_dtype, out_dtype, c.stream);
+}
+
+int dtas_gemv_w4(const void* x, const float* x_scale, const void* w, const void* w_scale, const void* w_zero,
+                 const void* bias, const void* res1, const void* res2, void* y, int64_t m, int64_t n, int64_t k,
+                 int64_t group, int act, int x_dtype, int out_dtype, int device, void* stream) {
+  DTAS_NONNULL("gemv_w4", x);
+  DTAS_NONNULL("gemv_w4", w);
+  DTAS_NONNULL("gemv_w4", w_scale);
+  DTAS_NONNULL("gemv_w4", y);
+  if (m <= 0 || n <= 0 || k <= 0)
+    DTAS_FAIL(DTAS_EINVAL, "gemv_w4: m, n and k must be > 0, got m=%lld n=%lld k=%lld", (long long)m, (long long)n, (long long)k);
+  if (m > DTAS_W4_MAX_ROWS)
+    DTAS_FAIL(DTAS_EUNSUPPORTED, "gemv_w4: at most %d rows, got %lld", DTAS_W4_MAX_ROWS, (long long)m);
+  if (n > 0x7fffffffLL - 16 || k > 0x7fffffffLL / 2) DTAS_FAIL(DTAS_EINVAL, "gemv_w4: n or k too large");
+  if (k % 2 != 0) DTAS_FAIL(DTAS_EINVAL, "gemv_w4: k must be even, got %lld", (long long)k);
+  if (group <= 0 || k % group != 0)
+    DTAS_FAIL(DTAS_EINVAL, "gemv_w4: the group size (%lld) must divide k (%lld)", (long long)group, (long long)k);
+  if (x_dtype != DTAS_F16 && x_dtype != DTAS_I8 && x_dtype != DTAS_E4M3)
+    DTAS_FAIL(DTAS_EUNSUPPORTED, "gemv_w4: x is fp16, int8 or e4m3 (dtype %d)", x_dtype);
+  if ((x_dtype == DTAS_F16) != (x_scale == nullptr))
+    DTAS_FAIL(DTAS_EINVAL, "gemv_w4: x_scale belongs to an x of 8 bits, and only to one");
+  int rc;
+  if ((rc = check_epilogue("gemv_w4", act, out_dtype))) return rc;
+  if (res1 == nullptr && res2 != nullptr) DTAS_FAIL(DTAS_EINVAL, "gemv_w4: res2 without res1");
+  Call c;
+  if ((rc = c.begin(device, stream))) return rc;
+  Epilogue epi;
+  epi.bias = static_cast<const __half*>(bias);
+  epi.res1 = static_cast<const __half*>(res1);
+  epi.res2 = static_cast<const __half*>(res2);
+  epi.ldr = n;
+  epi.act = act;
+  epi.out_f32 = out_dtype == DTAS_F32 ? 1 : 0;
+  return launch_gemv_w4(x, x_scale, w, w_scale, w_zero, epi, y, m, n, k, group, x_dtype, c.stream);
+}
+
+int dtas_gemm_nt_f8(const void* x, const void* w, const float* x_scale, const float* w_scale, const void* bias,
+                    const void* res1, const void* res2, void* y, int64_t m, int64_t n, int64_t k, int64_t ldy,
+                    int64_t ldr, int act, int out_dtype, int device, void* stream) {
+  DTAS_NONNULL("gemm_f8", x);
+  DTAS_NONNULL("gemm_f8", w);
+  DTAS_NONNULL("gemm_f8", x_scale);
+  DTAS_NONNULL("gemm_f8", w_scale);
+  DTAS_NONNULL("gemm_f8", y);
+  if (m <= 0) DTAS_FAIL(DTAS_EINVAL, "gemm_f8: dynamic dim m must be > 0, got %lld", (long long)m);
+  if (n <= 0 || k <= 0)
+    DTAS_FAIL(DTAS_EINVAL, "gemm_f8: n and k must be > 0, got n=%lld k=%lld", (long long)n, (long long)k);
+  if (ldy < n) DTAS_FAIL(DTAS_EINVAL, "gemm_f8: ldy (%lld) must be >= n (%lld)", (long long)ldy, (long long)n);
+  int rc;
+  if ((rc = check_epilogue("gemm_f8", act, out_dtype))) return rc;
+  if (res1 == nullptr && res2 != nullptr) DTAS_FAIL(DTAS_EINVAL, "gemm_f8: res2 without res1");
+  if (res1 != nullptr && ldr < n)
+    DTAS_FAIL(DTAS_EINVAL, "gemm_f8: ldr (%lld) must be >= n (%lld)", (long long)ldr, (long long)n);
+  Call c;
+  if ((rc = c.begin(device, stream))) return rc;
+  Epilogue epi;
+  epi.bias = static_cast<const __half*>(bias);
+  epi.res1 = static_cast<const __half*>(res1);
+  epi.res2 = static_cast<const __half*>(res2);
+  epi.ldr = res1 != nullptr ? ldr : 0;
+  epi.act = act;
+  epi.out_f32 = out_dtype == DTAS_F32 ? 1 : 0;
+  epi.sx = x_scale;
+  epi.sw = w_scale;
+  return launch_gemm(x, w, epi, y, m, n, k, ldy, c.ctx, c.stream, nullptr, true);
+}
+
 int dtas_gemm_nt_scatter(const void* x, const void* w, const void* bias, void* y, void* const* peer_ys, int n_peers,
                          int64_t m, int64_t n, int64_t k, int64_t ldy, int dtype, int device, void* stream) {
   return dtas_gemm_nt_scatter_multicast(x, w, bias, y, peer_ys, n_peers, nullptr, m, n, k, ldy, dtype, device, stream);
@@ -359,7 +458,10 @@ int dtas_variant_of(const char* op, int64_t m, int64_t n, int64_t k, int device,
     case 4: row_variant_name(ROW_SOFTMAX, m, n, buf, buf_len); break;
     case 5: row_variant_name(ROW_LAYERNORM, m, n, buf, buf_len); break;
     case 6: gemv_variant_name(n, k, ctx, buf, buf_len); break;
-    default: gemm_variant_name(m, n, k, ctx, buf, buf_len); break;
+    case 7: gemm_variant_name(m, n, k, ctx, buf, buf_len); break;
+    case 8: case 9: row_quant_variant_name(op, m, n, buf, buf_len); break;
+    case 10: gemv_w4_variant_name(m, n, k, buf, buf_len); break;
+    default: gemm_f8_variant_name(m, n, k, ctx, buf, buf_len); break;
   }
   return DTAS_OK;
 }

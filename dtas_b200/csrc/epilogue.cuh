@@ -8,7 +8,8 @@
 // decode-time GEMV forms at :96-114, 408-440, 442-481, 483-550).  The reference rounds every
 // intermediate to fp16; here the chain is evaluated in fp32 on the fp32 accumulator and rounded
 // to fp16 once, which is the closer of the two to exact arithmetic.  An fp32 output holds that
-// fp16 value widened, as the reference's trailing cast does.
+// fp16 value widened, as the reference's trailing cast does.  Products of 8-bit operands bring their scales,
+// one per row of X and one per row of W, in front of the chain.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -26,6 +27,8 @@ struct Epilogue {
   int act = DTAS_ACT_NONE;
   int out_f32 = 0;                // 0: Y is fp16, 1: Y is fp32
   int vec_res = 0;                // 16-byte loads from residual rows are aligned (set by the launcher)
+  const float* sx = nullptr;      // 8-bit operands: scale of every row of X [m] ...
+  const float* sw = nullptr;      //   ... and of every row of W [n]; both or neither
 };
 
 // Further copies of Y: base pointers of buffers with Y's layout (same row stride, same dtype) in which
@@ -42,7 +45,9 @@ struct PeerOut {
 };
 
 // Host and device: true when finishing an element costs more than a bias add and a store.
-inline __host__ __device__ bool epi_has_work(const Epilogue& e) { return e.act != DTAS_ACT_NONE || e.res1 != nullptr; }
+inline __host__ __device__ bool epi_has_work(const Epilogue& e) {
+  return e.act != DTAS_ACT_NONE || e.res1 != nullptr || e.sx != nullptr;
+}
 
 #ifdef __CUDACC__
 // GELU, erf form: x * (0.5 + 0.5 * erf(x / sqrt(2))), as the reference's workload spells it
@@ -100,6 +105,7 @@ __device__ __forceinline__ float epi_tail(const Epilogue& e, float t, int64_t ro
 }
 // Value of one output element from its fp32 dot product.
 __device__ __forceinline__ float epi_value(const Epilogue& e, float acc, int64_t row, int col) {
+  if (e.sx != nullptr) acc = acc * e.sx[row] * e.sw[col];
   if (e.bias != nullptr) acc += __half2float(e.bias[col]);
   return epi_tail(e, acc, row, col);
 }
@@ -108,6 +114,18 @@ __device__ __forceinline__ void epi_store(const Epilogue& e, void* y, int64_t ld
   const __half h = __float2half_rn(v);
   if (e.out_f32) static_cast<float*>(y)[row * ldy + col] = __half2float(h);
   else static_cast<__half*>(y)[row * ldy + col] = h;
+}
+
+// Scales of 8-bit operands and the bias on COUNT consecutive rows of one output column, in place.
+template <int COUNT>
+__device__ __forceinline__ void epi_scale_bias_column(const Epilogue& e, int row0, int m, int col, float bias, float* v) {
+  if (e.sx != nullptr) {
+    const float sw = e.sw[col];
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) v[j] = v[j] * (row0 + j < m ? e.sx[row0 + j] : 0.f) * sw;
+  }
+#pragma unroll
+  for (int j = 0; j < COUNT; ++j) v[j] += bias;
 }
 
 // COUNT consecutive rows row0, row0+1, ... of one output column; v[] holds dot product + bias.
@@ -214,7 +232,7 @@ __device__ __forceinline__ void epi_add_res32(const __half* res, int64_t off, in
 // True when the tail is nothing but an optional bias and an fp16 store: the path every plain GEMM
 // takes, kept free of the machinery below.
 __device__ __forceinline__ bool epi_is_plain(const Epilogue& e) {
-  return e.res1 == nullptr && e.act == DTAS_ACT_NONE && !e.out_f32;
+  return e.res1 == nullptr && e.act == DTAS_ACT_NONE && !e.out_f32 && e.sx == nullptr;
 }
 // The plain tail for 32 consecutive columns of one row, from the raw accumulator words.
 __device__ __forceinline__ void epi_store_row32_plain(const __half* bias, __half* yrow, int vec_store, int col0, int n,
@@ -253,10 +271,31 @@ __device__ __forceinline__ void epi_store_row32_plain(const __half* bias, __half
   }
 }
 
-// The arithmetic of the tail on 32 consecutive columns of one row, in place: bias, activation,
-// residuals.  `pre`, when given, holds the residual values of this chunk fetched earlier.
+// The scales of 8-bit operands on 32 consecutive columns of one row.
+__device__ __forceinline__ void epi_scale_row32(const Epilogue& e, int64_t row, int col0, int n, float* acc32) {
+  const float sx = e.sx[row];
+  if (col0 + 32 <= n && (reinterpret_cast<uintptr_t>(e.sw + col0) & 15) == 0) {
+    const float4* src = reinterpret_cast<const float4*>(e.sw + col0);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const float4 v = __ldg(src + q);
+      acc32[4 * q] = acc32[4 * q] * sx * v.x;
+      acc32[4 * q + 1] = acc32[4 * q + 1] * sx * v.y;
+      acc32[4 * q + 2] = acc32[4 * q + 2] * sx * v.z;
+      acc32[4 * q + 3] = acc32[4 * q + 3] * sx * v.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (col0 + j < n) acc32[j] = acc32[j] * sx * e.sw[col0 + j];
+  }
+}
+
+// The arithmetic of the tail on 32 consecutive columns of one row, in place: scales of 8-bit operands, bias,
+// activation, residuals.  `pre`, when given, holds the residual values of this chunk fetched earlier.
 __device__ __forceinline__ void epi_apply_row32(const Epilogue& e, int64_t row, int col0, int n, float* acc32,
                                                 const ResChunk* pre = nullptr) {
+  if (e.sx != nullptr) epi_scale_row32(e, row, col0, n, acc32);
   if (e.bias != nullptr) epi_add_bias32(e.bias, col0, n, acc32);
   if (e.act == DTAS_ACT_GELU) {
 #pragma unroll

@@ -35,7 +35,12 @@
 //
 // Work per launch: 2*m*n*k flop; bytes 2*(m*k + n*k + m*n).  Bound: tensor pipe for
 // m >= ~1024, HBM (W stream) for small m.
+//
+// The same kernels compute the product of e4m3 operands with a scale per row of X and per row of W
+// (dtas_gemm_nt_f8; GemmArgs::f8): the issuing thread uses the f8f6f4 kind of the instruction, which takes
+// 32 elements where the fp16 kind takes 16, and the epilogue starts with the scales.
 #include <cuda.h>
+#include <cuda_fp8.h>
 
 #include <mutex>
 #include <vector>
@@ -137,18 +142,45 @@ __device__ __forceinline__ void tc_fence_before() {
 __device__ __forceinline__ void tc_fence_after() {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
-// D[tmem] (+)= A[smem desc] * B[smem desc]; accumulate == 0 overwrites D.
-__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
-                                         uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t"
-      ".reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
-      "}"
-      :
-      : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
+// D[tmem] (+)= A[smem desc] * B[smem desc]; accumulate == 0 overwrites D.  F8: e4m3 operands.  To everything
+// but this instruction an e4m3 row of K elements is a row of K / 2 16-bit words: a k-block is 128 bytes of a
+// row, an MMA takes 32 bytes of it (16 fp16 or 32 e4m3 elements) in the same time, and in the
+// instruction descriptor both element formats have code 0 of their kind.
+template <bool F8>
+__device__ __forceinline__ void umma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                     uint32_t accumulate) {
+  if constexpr (F8) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+        "}"
+        :
+        : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+        "}"
+        :
+        : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
+}
+// The MMAs of one k-block (one 128-byte swizzle row of both operands).
+__device__ __forceinline__ void umma_kblock(int f8, uint32_t d_tmem, uint64_t da, uint64_t db, uint32_t idesc, bool first) {
+  // advancing 16 fp16 or 32 e4m3 along K inside the swizzle row = +32 bytes = +2 in the address field
+  if (f8) {
+#pragma unroll
+    for (int kk = 0; kk < BK / UMMA_K; ++kk) umma<true>(d_tmem, da + 2u * kk, db + 2u * kk, idesc, (!first || kk > 0) ? 1u : 0u);
+  } else {
+#pragma unroll
+    for (int kk = 0; kk < BK / UMMA_K; ++kk) umma<false>(d_tmem, da + 2u * kk, db + 2u * kk, idesc, (!first || kk > 0) ? 1u : 0u);
+  }
 }
 // Arrives on the mbarrier once every tcgen05.mma issued so far by this thread has retired.
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
@@ -217,6 +249,7 @@ struct GemmArgs {
   int sk_first = 0;   // two-CTA kernel, stream-K: first tile of the region that is cut into runs of units
   int slots_cap = 0;  // partial-tile slots reserved per output tile in the workspace
   PeerOut peers;      // two-CTA kernel: further buffers that receive every stored vector of Y
+  int f8 = 0;         // 1: X and W are e4m3, two elements to a 16-bit word of k (epi.sx / epi.sw scale the result)
 };
 
 template <int BN>
@@ -391,11 +424,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           const uint32_t sa = base + stage * C::kStageBytes;
           const uint64_t da = make_kmajor_sw128_desc(sa);
           const uint64_t db = make_kmajor_sw128_desc(sa + C::kABytes);
-#pragma unroll
-          for (int kk = 0; kk < BK / UMMA_K; ++kk) {
-            // advancing 16 fp16 along K inside the swizzle row = +32 bytes = +2 in the address field
-            umma_f16(d_tmem, da + 2u * kk, db + 2u * kk, idesc, (kb > kb0 || kk > 0) ? 1u : 0u);
-          }
+          umma_kblock(a.f8, d_tmem, da, db, idesc, kb == kb0);
           umma_commit(empty_bar(stage));   // stage reusable once these MMAs have read it
           if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
         }
@@ -768,9 +797,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           const uint32_t sa = base + stage * C::kStageBytes;
           const uint64_t da = make_kmajor_sw128_desc(sa);                // W rows: the M side
           const uint64_t db = make_kmajor_sw128_desc(sa + C::kWBytes);   // X rows: the N side
-#pragma unroll
-          for (int kk = 0; kk < BK / UMMA_K; ++kk)
-            umma_f16(d_tmem, da + 2u * kk, db + 2u * kk, idesc, (kb > kb0 || kk > 0) ? 1u : 0u);
+          umma_kblock(a.f8, d_tmem, da, db, idesc, kb == kb0);
           umma_commit(empty_bar(stage));
           if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
         }
@@ -808,7 +835,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           if (col_ok) {
             float f[kChunk];
 #pragma unroll
-            for (int j = 0; j < kChunk; ++j) f[j] = __uint_as_float(r[j]) + bias;
+            for (int j = 0; j < kChunk; ++j) f[j] = __uint_as_float(r[j]);
+            epi_scale_bias_column<kChunk>(a.epi, c * kChunk, a.m, col, bias, f);
             epi_store_column<kChunk>(a.epi, a.y, a.ldy, c * kChunk, a.m, col, f);
           }
         }
@@ -889,9 +917,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
               float o[4 * G];
 #pragma unroll
               for (int j = 0; j < G; ++j) {
-                o[4 * j] = sum4[j].x + bias; o[4 * j + 1] = sum4[j].y + bias;
-                o[4 * j + 2] = sum4[j].z + bias; o[4 * j + 3] = sum4[j].w + bias;
+                o[4 * j] = sum4[j].x; o[4 * j + 1] = sum4[j].y;
+                o[4 * j + 2] = sum4[j].z; o[4 * j + 3] = sum4[j].w;
               }
+              epi_scale_bias_column<4 * G>(a.epi, g0 * 4, a.m, col, bias, o);
               epi_store_column<4 * G>(a.epi, a.y, a.ldy, g0 * 4, a.m, col, o);
             }
           }
@@ -960,17 +989,39 @@ __device__ __forceinline__ void tmem_relinquish_pair() {
 __device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t cols) {
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
 }
-__device__ __forceinline__ void umma_f16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                              uint32_t accumulate) {
-  asm volatile(
-      "{\n\t"
-      ".reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t"
-      "}"
-      :
-      : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
+template <bool F8>
+__device__ __forceinline__ void umma_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t accumulate) {
+  if constexpr (F8) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+        "}"
+        :
+        : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t"
+        "}"
+        :
+        : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
+}
+__device__ __forceinline__ void umma_kblock_pair(int f8, uint32_t d_tmem, uint64_t da, uint64_t db, uint32_t idesc, bool first) {
+  if (f8) {
+#pragma unroll
+    for (int kk = 0; kk < BK / UMMA_K; ++kk) umma_pair<true>(d_tmem, da + 2u * kk, db + 2u * kk, idesc, (!first || kk > 0) ? 1u : 0u);
+  } else {
+#pragma unroll
+    for (int kk = 0; kk < BK / UMMA_K; ++kk) umma_pair<false>(d_tmem, da + 2u * kk, db + 2u * kk, idesc, (!first || kk > 0) ? 1u : 0u);
+  }
 }
 // Arrives on the barrier at this offset in every CTA of `cta_mask` once the MMAs issued so far retire.
 __device__ __forceinline__ void umma_commit_pair(uint32_t bar, uint16_t cta_mask) {
@@ -1188,9 +1239,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairMaxThreads, 1)
           const uint32_t sa = base + stage * kPairStageBytes;
           const uint64_t da = make_kmajor_sw128_desc(sa);
           const uint64_t db = make_kmajor_sw128_desc(sa + kPairHalfBytes);
-#pragma unroll
-          for (int kk = 0; kk < BK / UMMA_K; ++kk)
-            umma_f16_pair(d_tmem, da + 2u * kk, db + 2u * kk, idesc, (kb > sg.kb0 || kk > 0) ? 1u : 0u);
+          umma_kblock_pair(a.f8, d_tmem, da, db, idesc, kb == sg.kb0);
           umma_commit_pair(empty_bar(stage), 0x3);
           if (++stage == kPairStages) { stage = 0; phase ^= 1u; }
         }
@@ -1553,9 +1602,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
         const uint32_t sa = base + stage * C::kStageBytes;
         const uint64_t da = make_kmajor_sw128_desc(sa);
         const uint64_t db = make_kmajor_sw128_desc(sa + C::kABytes);
-#pragma unroll
-        for (int kk = 0; kk < BK / UMMA_K; ++kk)
-          umma_f16(tmem_base, da + 2u * kk, db + 2u * kk, idesc, (kb > kb0 || kk > 0) ? 1u : 0u);
+        umma_kblock(a.f8, tmem_base, da, db, idesc, kb == kb0);
         umma_commit(empty_bar(stage));
         if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
       }
@@ -1723,9 +1770,7 @@ __global__ void __cluster_dims__(S, 1, 1) __launch_bounds__(kGemmThreads, 1)
         const uint32_t sa = base + stage * C::kStageBytes;
         const uint64_t da = make_kmajor_sw128_desc(sa);
         const uint64_t db = make_kmajor_sw128_desc(sa + C::kWBytes);
-#pragma unroll
-        for (int kk = 0; kk < BK / UMMA_K; ++kk)
-          umma_f16(tmem_base, da + 2u * kk, db + 2u * kk, idesc, (kb > kb0 || kk > 0) ? 1u : 0u);
+        umma_kblock(a.f8, tmem_base, da, db, idesc, kb == kb0);
         umma_commit(empty_bar(stage));
         if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
       }
@@ -1787,8 +1832,7 @@ __global__ void __cluster_dims__(S, 1, 1) __launch_bounds__(kGemmThreads, 1)
                 f[4 * q] += v.x; f[4 * q + 1] += v.y; f[4 * q + 2] += v.z; f[4 * q + 3] += v.w;
               }
             }
-#pragma unroll
-            for (int j = 0; j < kChunk; ++j) f[j] += bias;
+            epi_scale_bias_column<kChunk>(a.epi, c * kChunk, a.m, col, bias, f);
             epi_store_column<kChunk>(a.epi, a.y, a.ldy, c * kChunk, a.m, col, f);
           }
         }
@@ -1808,18 +1852,21 @@ __global__ void __cluster_dims__(S, 1, 1) __launch_bounds__(kGemmThreads, 1)
 // SIMT fallback for shapes TMA cannot describe (k % 8 != 0 or unaligned bases): one thread
 // per output element, fp32 accumulation.  Correct for every shape, not a performance path.
 // ---------------------------------------------------------------------------------------
+__device__ __forceinline__ float simt_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float simt_f32(__nv_fp8_e4m3 v) { return (float)v; }
+template <typename T>
 __global__ void __launch_bounds__(256)
-    gemm_f16_simt_kernel(const __half* __restrict__ x, const __half* __restrict__ w, const Epilogue epi,
+    gemm_simt_kernel(const T* __restrict__ x, const T* __restrict__ w, const Epilogue epi,
                          void* __restrict__ y, int m, int n, int k, int64_t ldy) {
   const int col = blockIdx.x * 16 + (threadIdx.x & 15);
   const int row = blockIdx.y * 16 + (threadIdx.x >> 4);
   pdl_wait();
   pdl_launch_dependents();
   if (row >= m || col >= n) return;
-  const __half* xr = x + (int64_t)row * k;
-  const __half* wr = w + (int64_t)col * k;
+  const T* xr = x + (int64_t)row * k;
+  const T* wr = w + (int64_t)col * k;
   float acc = 0.f;
-  for (int i = 0; i < k; ++i) acc = fmaf(__half2float(xr[i]), __half2float(wr[i]), acc);
+  for (int i = 0; i < k; ++i) acc = fmaf(simt_f32(xr[i]), simt_f32(wr[i]), acc);
   epi_store(epi, y, ldy, row, col, epi_value(epi, acc, row, col));
 }
 
@@ -2534,9 +2581,21 @@ static int finish_epilogue(Epilogue& e, const void* y, int64_t ldy) {
 }
 
 int launch_gemm(const void* x, const void* w, const Epilogue& epi, void* y, int64_t m, int64_t n,
-                int64_t k, int64_t ldy, DeviceCtx* ctx, cudaStream_t st, const PeerOut* peers) {
+                int64_t k, int64_t ldy, DeviceCtx* ctx, cudaStream_t st, const PeerOut* peers, bool f8) {
   if (m > 0x7fffffffLL / 2 || n > 0x7fffffffLL / 2 || k > 0x7fffffffLL / 2)
     DTAS_FAIL(DTAS_EINVAL, "gemm: dimension too large");
+  if (f8) {
+    // e4m3 rows travel as rows of K / 2 16-bit words: tiles, rings, work distribution and the table see
+    // the fp16 product of that length, which moves the same bytes in the same MMA time
+    if (k % 16 != 0 || !aligned16(x) || !aligned16(w)) {
+      dim3 grid((unsigned)((n + 15) / 16), (unsigned)((m + 15) / 16));
+      if (grid.y > 65535) DTAS_FAIL(DTAS_EUNSUPPORTED, "gemm: unaligned operands with m > 1048560");
+      launch_kernel(gemm_simt_kernel<__nv_fp8_e4m3>, grid, 256, 0, st, (const __nv_fp8_e4m3*)x, (const __nv_fp8_e4m3*)w,
+                    epi, y, (int)m, (int)n, (int)k, ldy);
+      return after_launch("gemm_simt_kernel");
+    }
+    k /= 2;
+  }
   GemmPlan p = plan_gemm(m, n, k, ctx->sm_count, gemm_tma_ok(x, w, k));
   const bool scatter = peers != nullptr && peers->n > 0;
   if (scatter && !p.pair) {
@@ -2549,9 +2608,9 @@ int launch_gemm(const void* x, const void* w, const Epilogue& epi, void* y, int6
   if (p.simt) {
     dim3 grid((unsigned)((n + 15) / 16), (unsigned)((m + 15) / 16));
     if (grid.y > 65535) DTAS_FAIL(DTAS_EUNSUPPORTED, "gemm: unaligned operands with m > 1048560");
-    launch_kernel(gemm_f16_simt_kernel, grid, 256, 0, st, (const __half*)x, (const __half*)w, epi, y, (int)m,
+    launch_kernel(gemm_simt_kernel<__half>, grid, 256, 0, st, (const __half*)x, (const __half*)w, epi, y, (int)m,
                   (int)n, (int)k, ldy);
-    return after_launch("gemm_f16_simt_kernel");
+    return after_launch("gemm_simt_kernel");
   }
   float* ws = nullptr;
   int* counters = nullptr;
@@ -2583,6 +2642,7 @@ int launch_gemm(const void* x, const void* w, const Epilogue& epi, void* y, int6
   a.kb_per_split = p.kb_per_split;
   a.num_kb = (int)((k + BK - 1) / BK);
   a.vec_store = finish_epilogue(a.epi, y, ldy);
+  a.f8 = f8 ? 1 : 0;
   if (scatter) {
     a.peers = *peers;
     for (int j = 0; j < peers->n; ++j)
@@ -2628,6 +2688,15 @@ int launch_gemm(const void* x, const void* w, const Epilogue& epi, void* y, int6
     case 128: return launch_tc<128>(tx, tw, a, ctx->sm_count, st);
     default: return launch_tc<64>(tx, tw, a, ctx->sm_count, st);
   }
+}
+
+void gemm_f8_variant_name(int64_t m, int64_t n, int64_t k, const DeviceCtx* ctx, char* buf, int len) {
+  if (k % 16 != 0) {
+    snprintf(buf, len, "gemm_f8_simt_fallback");
+    return;
+  }
+  const int head = snprintf(buf, len, "f8_");
+  if (head < len) gemm_variant_name(m, n, k / 2, ctx, buf + head, len - head);
 }
 
 void gemm_variant_name(int64_t m, int64_t n, int64_t k, const DeviceCtx* ctx, char* buf, int len) {

@@ -1,0 +1,400 @@
+// Rows on their way into a low-bit projection: the residual's addition with the RMS norm, and rows
+// brought to 8 bits with one scale each (int8 or e4m3, symmetric).  No counterpart in the reference.
+//
+//   add_rms_norm : h = x + res (res optional), r = 1 / sqrt(mean(h^2) + eps), y = h * r * weight
+//   quantize     : y = x
+//   8-bit result : scale = max|y| / Q, q = round(y * Q / max|y|), Q = 448 (e4m3) or 127 (int8)
+//
+// r is the same for the whole row, so it cancels out of q: with u = h * weight,
+// q = round(u * Q / max|u|) and scale = r * max|u| / Q.  The sum of squares and max|u| are therefore
+// taken in ONE pass and meet in one exchange between the row's warps, where the formula as written
+// would need two (first r, then the maximum of what r scales).
+//
+// h is held in fp32 between the reduction and the result: the norm sees the exact sum of two fp16
+// values, not the rounded one that is stored as the new residual.
+//
+// Design: blockDim.x threads own a row and blockDim.y rows share a CTA; a thread holds CH chunks of VEC
+// consecutive elements, all loads in flight at once.  The threads per row are the row's chunks over CH,
+// rounded up to whole warps and not to a power of two, so that 11008 columns take 352 threads x 4 chunks
+// and none idles.  Bound: HBM; every element is read once and written once.
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace dtas {
+namespace {
+
+enum { Q_NORM = 0, Q_QUANT = 1 };
+constexpr int kMaxThreads = 1024;
+// Threads a CTA may have: what leaves a thread the registers for its chunks.
+constexpr int max_threads(int vec, int ch) { return vec * ch > 16 ? 512 : kMaxThreads; }
+
+struct RowArgs {
+  const void* x;
+  const void* res;       // optional (norm)
+  const __half* weight;  // norm
+  void* y;
+  void* res_out;         // optional (norm)
+  float* scale;          // 8-bit results
+  int64_t m;
+  int64_t n_cols;
+  float eps;
+};
+
+template <typename T>
+struct OutTraits;
+template <>
+struct OutTraits<__half> {
+  static constexpr float kQ = 0.f;
+};
+template <>
+struct OutTraits<int8_t> {
+  static constexpr float kQ = 127.f;
+};
+template <>
+struct OutTraits<__nv_fp8_e4m3> {
+  static constexpr float kQ = 448.f;
+};
+
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(float v) { return v; }
+
+// VEC consecutive elements of a row; VEC = 8 needs 16-byte aligned rows (32-byte pairs for fp32).
+template <int VEC, typename T>
+__device__ __forceinline__ void load_vec(const T* p, float* v) {
+  if constexpr (VEC == 8 && sizeof(T) == 2) {
+    const uint4 r = __ldcs(reinterpret_cast<const uint4*>(p));
+    const __half2* h = reinterpret_cast<const __half2*>(&r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(h[i]);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  } else if constexpr (VEC == 8) {
+    const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = to_f32(p[i]);
+  }
+}
+
+template <int VEC>
+__device__ __forceinline__ void store_vec(__half* p, const float* v) {
+  if constexpr (VEC == 8) {
+    __stcs(reinterpret_cast<uint4*>(p), epi_pack8(v));
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) p[i] = __float2half_rn(v[i]);
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void store_vec(float* p, const float* v) {
+  if constexpr (VEC == 8) {
+    __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
+    __stcs(reinterpret_cast<float4*>(p) + 1, make_float4(v[4], v[5], v[6], v[7]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) p[i] = v[i];
+  }
+}
+__device__ __forceinline__ uint32_t pack4(const float* v, int8_t) {
+  const int a = __float2int_rn(v[0]), b = __float2int_rn(v[1]), c = __float2int_rn(v[2]), d = __float2int_rn(v[3]);
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+__device__ __forceinline__ uint32_t pack4(const float* v, __nv_fp8_e4m3) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[0], v[1]), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[2], v[3]), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+// |v| <= Q up to the last rounding, so nothing here is clamped but by that rounding itself.
+template <int VEC, typename OutT>
+__device__ __forceinline__ void store_q(OutT* p, const float* v) {
+  if constexpr (VEC == 8) {
+    __stcs(reinterpret_cast<uint2*>(p), make_uint2(pack4(v, OutT{}), pack4(v + 4, OutT{})));
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      if constexpr (sizeof(OutT) == 1 && OutTraits<OutT>::kQ == 127.f)
+        p[i] = (int8_t)__float2int_rn(v[i]);
+      else
+        reinterpret_cast<__nv_fp8_storage_t*>(p)[i] = __nv_cvt_float_to_fp8(v[i], __NV_SATFINITE, __NV_E4M3);
+    }
+  }
+}
+
+// max that keeps a NaN, so that a row with one is not taken for a finite row
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Sum and maximum over the threads of one row (blockDim.x, a multiple of 32).  One exchange through shared
+// memory for both; `ex` holds two floats per warp of the CTA.  Rows of one warp need no exchange.
+__device__ __forceinline__ void row_reduce(float& sum, float& top, float2* ex) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+  }
+  const int nw = blockDim.x >> 5;
+  if (nw == 1) return;
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) ex[threadIdx.y * nw + (threadIdx.x >> 5)] = make_float2(sum, top);
+  __syncthreads();
+  const float2 e = lane < nw ? ex[threadIdx.y * nw + lane] : make_float2(0.f, 0.f);
+  sum = e.x;
+  top = e.y;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+  }
+}
+
+// What an element is multiplied by on its way to 8 bits, and the row's scale.  A maximum so small that
+// Q / top would overflow goes through two steps (`pre` then `mul`); a row of zeros gets q = 0; a row that
+// holds an infinity or a NaN gets a NaN scale, and so stands for NaN whatever its q.
+struct QuantMul {
+  float pre, mul;
+};
+__device__ __forceinline__ QuantMul quant_mul(float top, float q) {
+  if (!(top < INFINITY)) return {0.f, 0.f};
+  if (top >= 0x1p-100f) return {1.f, q / top};
+  if (top > 0.f) return {0x1p100f, q / (top * 0x1p100f)};    // top * 2^100 is exact
+  return {0.f, 0.f};
+}
+__device__ __forceinline__ float quant_scale(float top, float r, float q) {
+  return top < INFINITY ? (top * r) / q : __int_as_float(0x7fc00000);
+}
+
+template <int OP, typename InT, typename OutT, int VEC, int CH>
+__global__ void __launch_bounds__(max_threads(VEC, CH)) row_quant_kernel(const RowArgs a) {
+  __shared__ float2 ex[kMaxThreads / 32];
+  constexpr bool kNorm = OP == Q_NORM;
+  constexpr bool k8 = sizeof(OutT) == 1;
+  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  const bool live = row < a.m;
+  const int n = (int)a.n_cols;
+  const int64_t off = (live ? row : 0) * a.n_cols;
+  const InT* x = static_cast<const InT*>(a.x) + off;
+
+  pdl_wait();
+  pdl_launch_dependents();
+  float v[CH][VEC];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int e = (c * blockDim.x + threadIdx.x) * VEC;
+    if (live && e < n) {
+      load_vec<VEC>(x + e, v[c]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[c][i] = 0.f;
+    }
+  }
+  float sum = 0.f, top = 0.f;
+  if constexpr (kNorm) {
+    if (a.res != nullptr) {
+      const InT* res = static_cast<const InT*>(a.res) + off;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int e = (c * blockDim.x + threadIdx.x) * VEC;
+        if (live && e < n) {
+          float t[VEC];
+          load_vec<VEC>(res + e, t);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) v[c][i] += t[i];
+        }
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) sum = fmaf(v[c][i], v[c][i], sum);
+      const int e = (c * blockDim.x + threadIdx.x) * VEC;
+      if (live && e < n) {
+        if (a.res_out != nullptr) store_vec<VEC>(static_cast<InT*>(a.res_out) + off + e, v[c]);
+        if constexpr (k8) {
+          float w[VEC];
+          load_vec<VEC>(a.weight + e, w);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) v[c][i] *= w[i];
+        }
+      }
+    }
+  }
+  if constexpr (k8) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) top = max_nan(top, fabsf(v[c][i]));
+  }
+  row_reduce(sum, top, ex);
+  if (!live) return;
+  float r = 1.f;
+  if constexpr (kNorm) r = 1.0f / sqrtf(sum / (float)n + a.eps);
+  OutT* y = static_cast<OutT*>(a.y) + off;
+  if constexpr (k8) {
+    const QuantMul qm = quant_mul(top, OutTraits<OutT>::kQ);
+    if (threadIdx.x == 0) a.scale[row] = quant_scale(top, r, OutTraits<OutT>::kQ);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int e = (c * blockDim.x + threadIdx.x) * VEC;
+      if (e < n) {
+        float q[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) q[i] = (v[c][i] * qm.pre) * qm.mul;
+        store_q<VEC>(y + e, q);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int e = (c * blockDim.x + threadIdx.x) * VEC;
+      if (e < n) {
+        float w[VEC];
+        load_vec<VEC>(a.weight + e, w);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) w[i] = __fmul_rn(__fmul_rn(v[c][i], r), w[i]);
+        store_vec<VEC>(reinterpret_cast<__half*>(y) + e, w);
+      }
+    }
+  }
+}
+
+// Rows longer than the registers of a CTA hold: one CTA per row, which passes over it twice (the second
+// time out of L2).  Every element of the results is written by the thread that has just read its inputs,
+// behind the only reduction, so results in place of inputs are fine here too.
+template <int OP, typename InT, typename OutT>
+__global__ void __launch_bounds__(kMaxThreads) row_quant_long_kernel(const RowArgs a) {
+  __shared__ float2 ex[kMaxThreads / 32];
+  constexpr bool kNorm = OP == Q_NORM;
+  constexpr bool k8 = sizeof(OutT) == 1;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t off = (int64_t)blockIdx.x * a.n_cols;
+  const InT* x = static_cast<const InT*>(a.x) + off;
+  const InT* res = kNorm && a.res != nullptr ? static_cast<const InT*>(a.res) + off : nullptr;
+  float sum = 0.f, top = 0.f;
+  for (int64_t i = threadIdx.x; i < a.n_cols; i += blockDim.x) {
+    float h = to_f32(x[i]);
+    if (kNorm && res != nullptr) h += to_f32(res[i]);
+    if constexpr (kNorm) {
+      sum = fmaf(h, h, sum);
+      if constexpr (k8) h *= __half2float(a.weight[i]);
+    }
+    if constexpr (k8) top = max_nan(top, fabsf(h));
+  }
+  row_reduce(sum, top, ex);
+  float r = 1.f;
+  if constexpr (kNorm) r = 1.0f / sqrtf(sum / (float)a.n_cols + a.eps);
+  const QuantMul qm = quant_mul(top, k8 ? OutTraits<OutT>::kQ : 1.f);
+  if (k8 && threadIdx.x == 0) a.scale[blockIdx.x] = quant_scale(top, r, OutTraits<OutT>::kQ);
+  OutT* y = static_cast<OutT*>(a.y) + off;
+  for (int64_t i = threadIdx.x; i < a.n_cols; i += blockDim.x) {
+    float h = to_f32(x[i]);
+    if (kNorm && res != nullptr) h += to_f32(res[i]);
+    const float w = kNorm ? __half2float(a.weight[i]) : 1.f;
+    if constexpr (kNorm) {
+      if (a.res_out != nullptr) store_vec<1>(static_cast<InT*>(a.res_out) + off + i, &h);
+    }
+    if constexpr (k8) {
+      const float u = kNorm ? h * w : h;
+      const float q = (u * qm.pre) * qm.mul;
+      store_q<1>(y + i, &q);
+    } else {
+      const float o = __fmul_rn(__fmul_rn(h, r), w);
+      store_vec<1>(reinterpret_cast<__half*>(y) + i, &o);
+    }
+  }
+}
+
+// ---- dispatch ------------------------------------------------------------------
+struct RowPlan {
+  int vec;       // 8, or 1 where a row's length or an address rules out 16-byte vectors; 0: the long kernel
+  int ch;        // chunks per thread
+  int tpr;       // threads per row
+  int rows;      // rows per CTA
+};
+
+inline RowPlan row_plan(int64_t m, int64_t n_cols, bool vec_ok) {
+  RowPlan p{0, 0, 0, 0};
+  p.vec = vec_ok ? 8 : 1;
+  const int64_t chunks = (n_cols + p.vec - 1) / p.vec;
+  const int64_t most = vec_ok ? 8 * max_threads(8, 8) : 16 * max_threads(1, 16);
+  if (chunks > most) {
+    p.vec = 0;
+    p.tpr = kMaxThreads;
+    p.rows = 1;
+    return p;
+  }
+  if (vec_ok) p.ch = m <= 592 && chunks <= kMaxThreads ? 1 : (chunks <= 64 ? 2 : (chunks <= 2048 ? 4 : 8));
+  else p.ch = chunks <= 256 * 4 ? 4 : 16;
+  p.tpr = (int)((chunks + p.ch - 1) / p.ch + 31) / 32 * 32;
+  p.rows = p.tpr >= 256 ? 1 : 256 / p.tpr;
+  return p;
+}
+
+template <int OP, typename InT, typename OutT>
+int launch_typed(const RowPlan& p, const RowArgs& a, cudaStream_t st) {
+  const dim3 block(p.tpr, p.rows);
+  const int64_t grid = (a.m + p.rows - 1) / p.rows;
+  if (grid > 0x7fffffffLL) DTAS_FAIL(DTAS_EINVAL, "row op: too many rows (%lld)", (long long)a.m);
+  if (p.vec == 0) {
+    launch_kernel(row_quant_long_kernel<OP, InT, OutT>, (unsigned)grid, block, 0, st, a);
+    return after_launch("row_quant_long_kernel");
+  }
+#define DTAS_ROWQ_CASE(V, C)                                                                       \
+  if (p.vec == V && p.ch == C) {                                                                   \
+    launch_kernel(row_quant_kernel<OP, InT, OutT, V, C>, (unsigned)grid, block, 0, st, a);         \
+    return after_launch("row_quant_kernel");                                                       \
+  }
+  DTAS_ROWQ_CASE(8, 1) DTAS_ROWQ_CASE(8, 2) DTAS_ROWQ_CASE(8, 4) DTAS_ROWQ_CASE(8, 8)
+  DTAS_ROWQ_CASE(1, 4) DTAS_ROWQ_CASE(1, 16)
+#undef DTAS_ROWQ_CASE
+  DTAS_FAIL(DTAS_EINVAL, "row op: no kernel for %d x %d", p.vec, p.ch);
+}
+
+template <int OP, typename InT>
+int launch_out(const RowPlan& p, const RowArgs& a, int out_dtype, cudaStream_t st) {
+  if (out_dtype == DTAS_E4M3) return launch_typed<OP, InT, __nv_fp8_e4m3>(p, a, st);
+  if (out_dtype == DTAS_I8) return launch_typed<OP, InT, int8_t>(p, a, st);
+  if constexpr (OP == Q_NORM) {
+    if (out_dtype == DTAS_F16) return launch_typed<OP, InT, __half>(p, a, st);
+  }
+  DTAS_FAIL(DTAS_EUNSUPPORTED, "row op: unsupported output dtype %d", out_dtype);
+}
+
+template <int OP>
+int launch_in(const RowArgs& a, int in_dtype, int out_dtype, cudaStream_t st) {
+  bool vec_ok = a.n_cols % 8 == 0 && aligned16(a.x) && aligned16(a.res) && aligned16(a.weight) && aligned16(a.res_out);
+  vec_ok = vec_ok && (reinterpret_cast<uintptr_t>(a.y) & (out_dtype == DTAS_F16 ? 15 : 7)) == 0;
+  const RowPlan p = row_plan(a.m, a.n_cols, vec_ok);
+  if (in_dtype == DTAS_F16) return launch_out<OP, __half>(p, a, out_dtype, st);
+  if (in_dtype == DTAS_F32) return launch_out<OP, float>(p, a, out_dtype, st);
+  DTAS_FAIL(DTAS_EUNSUPPORTED, "row op: unsupported input dtype %d", in_dtype);
+}
+
+}  // namespace
+
+int launch_add_rms_norm(const void* x, const void* res, const void* weight, void* y, void* res_out, float* scale,
+                        int64_t m, int64_t n_cols, float eps, int in_dtype, int out_dtype, cudaStream_t st) {
+  return launch_in<Q_NORM>(RowArgs{x, res, static_cast<const __half*>(weight), y, res_out, scale, m, n_cols, eps},
+                           in_dtype, out_dtype, st);
+}
+
+int launch_quantize(const void* x, void* q, float* scale, int64_t m, int64_t n_cols, int in_dtype, int out_dtype,
+                    cudaStream_t st) {
+  return launch_in<Q_QUANT>(RowArgs{x, nullptr, nullptr, q, nullptr, scale, m, n_cols, 0.f}, in_dtype, out_dtype, st);
+}
+
+void row_quant_variant_name(const char* op, int64_t m, int64_t n_cols, char* buf, int len) {
+  const RowPlan p = row_plan(m, n_cols, n_cols % 8 == 0);
+  if (p.vec == 0) snprintf(buf, len, "%s_long_cta%d", op, p.tpr);
+  else snprintf(buf, len, "%s_vec%d_tpr%d_ch%d", op, p.vec, p.tpr, p.ch);
+}
+
+}  // namespace dtas

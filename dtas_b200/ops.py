@@ -21,6 +21,7 @@ def _lib():
     return _L
 
 _DTYPE_CODE = {torch.float16: _abi.F16, torch.float32: _abi.F32, torch.int8: _abi.I8}
+_LOW_CODE = {torch.int8: _abi.I8, torch.float8_e4m3fn: _abi.E4M3}
 
 
 def _chk(status):
@@ -270,6 +271,121 @@ def gemm_nt_scatter(x, w, out, peers, bias=None, multicast=0):
     ptrs = (ctypes.c_void_p * len(peers))(*[p.data_ptr() for p in peers])
     _chk(_lib().dtas_gemm_nt_scatter_multicast(x.data_ptr(), w.data_ptr(), _ptr(bias), out.data_ptr(), ptrs, len(peers),
                                                int(multicast) or None, m, n, k, ldy, _abi.F16, dev, _raw_stream(dev)))
+    return out
+
+
+def _row_scale(name, what, t, rows):
+    if t is None or t.dtype != torch.float32 or t.numel() != rows:
+        raise _abi.DtasError(_abi.EINVAL, f"{name}: {what} must be an fp32 vector of {rows} elements")
+
+
+def add_rms_norm(x, res, weight, out, res_out=None, scale=None, eps=1e-6):
+    """h = x + res; out = h * rsqrt(mean(h^2, -1) + eps) * weight; res_out = h.  One launch, fp32 arithmetic.
+
+    x and res are fp16 or fp32 of one dtype, weight is fp16 [H]; res may be None (h = x).  `res_out`, when given,
+    has x's dtype and may be x or res itself.  `out` is fp16, or int8 / float8_e4m3fn: then `scale`, fp32 [m],
+    receives max|row| / Q (Q = 127 or 448) and out holds the row over its scale, rounded to even.  A row
+    of zeros gets scale 0; a row with an infinity or a NaN gets a NaN scale."""
+    tensors = [t for t in (x, res, weight, out, res_out, scale) if t is not None]
+    dev, st = _check("add_rms_norm", *tensors)
+    m, h = _rows_cols(x, "add_rms_norm")
+    for t in (res, res_out):
+        if t is not None:
+            _same_shape("add_rms_norm", x, t)
+            if t.dtype != x.dtype:
+                raise _abi.DtasError(_abi.EINVAL, "add_rms_norm: res and res_out must have x's dtype")
+    _same_shape("add_rms_norm", x, out)
+    if weight.dtype != torch.float16 or weight.numel() != h:
+        raise _abi.DtasError(_abi.EINVAL, "add_rms_norm: weight must be fp16 [H]")
+    if out.dtype == torch.float16:
+        code, scale = _abi.F16, None
+    else:
+        code = _LOW_CODE.get(out.dtype)
+        if code is None:
+            raise _abi.DtasError(_abi.EUNSUPPORTED, f"add_rms_norm: out must be fp16, int8 or float8_e4m3fn, got {out.dtype}")
+        _row_scale("add_rms_norm", "scale", scale, m)
+    _chk(_lib().dtas_add_rms_norm(x.data_ptr(), _ptr(res), weight.data_ptr(), out.data_ptr(), _ptr(res_out), _ptr(scale),
+                                  m, h, float(eps), _code(x), code, dev, st))
+    return out
+
+
+def quantize(x, out, scale):
+    """Rows of x (fp16 or fp32) as int8 or float8_e4m3fn in `out` with one scale each in `scale` (fp32 [m]), as
+    add_rms_norm writes them: for activations that no norm precedes, and for the weights of gemm_nt_f8 (a
+    scale per output column)."""
+    dev, st = _check("quantize", x, out, scale)
+    _same_shape("quantize", x, out)
+    m, h = _rows_cols(x, "quantize")
+    code = _LOW_CODE.get(out.dtype)
+    if code is None:
+        raise _abi.DtasError(_abi.EUNSUPPORTED, f"quantize: out must be int8 or float8_e4m3fn, got {out.dtype}")
+    _row_scale("quantize", "scale", scale, m)
+    _chk(_lib().dtas_quantize(x.data_ptr(), out.data_ptr(), scale.data_ptr(), m, h, _code(x), code, dev, st))
+    return out
+
+
+def gemv_w4(x, w, w_scale, out, w_zero=None, x_scale=None, bias=None, res1=None, res2=None, act=None):
+    """out[m, N] = act(x[m, K] @ W[N, K]^T + bias[N]) + res1 + res2 for up to 16 rows, W in 4 bits:
+    W[n, k] = w_scale[n, k // G] * (code - w_zero[n, k // G]).
+
+    `w` is uint8 [N, K / 2], two codes to a byte, the even k in the low half; `w_scale` fp16 [N, K / G] says
+    what G is; `w_zero` uint8 of the same shape, 8 everywhere when None (dtas_b200.weights.quantize_w4
+    makes all three).  x is fp16, or int8 / float8_e4m3fn with x_scale fp32 [m], as add_rms_norm and
+    quantize write them.  out is fp16 or fp32 (the fp16 result widened); the tail is that of gemv."""
+    tensors = [t for t in (x, w, w_scale, out, w_zero, x_scale, bias, res1, res2) if t is not None]
+    dev, st = _check("gemv_w4", *tensors)
+    m, k = _rows_cols(x, "gemv_w4")
+    mo, n = _rows_cols(out, "gemv_w4")
+    if w.dtype != torch.uint8 or w.dim() != 2 or mo != m or tuple(w.shape) != (n, k // 2) or k % 2:
+        raise _abi.DtasError(_abi.EINVAL, f"gemv_w4: shapes x{tuple(x.shape)} w{tuple(w.shape)} out{tuple(out.shape)}; w is uint8 [N, K / 2]")
+    groups = int(w_scale.shape[1]) if w_scale.dim() == 2 else 0
+    if w_scale.dtype != torch.float16 or groups < 1 or int(w_scale.shape[0]) != n or k % groups:
+        raise _abi.DtasError(_abi.EINVAL, f"gemv_w4: w_scale must be fp16 [N, groups] with groups a divisor of K, got {tuple(w_scale.shape)}")
+    if w_zero is not None and (w_zero.dtype != torch.uint8 or w_zero.shape != w_scale.shape):
+        raise _abi.DtasError(_abi.EINVAL, "gemv_w4: w_zero must be uint8 with w_scale's shape")
+    if x.dtype == torch.float16:
+        x_code = _abi.F16
+        if x_scale is not None:
+            raise _abi.DtasError(_abi.EINVAL, "gemv_w4: x_scale belongs to an x of 8 bits")
+    else:
+        x_code = _LOW_CODE.get(x.dtype)
+        if x_code is None:
+            raise _abi.DtasError(_abi.EUNSUPPORTED, f"gemv_w4: x must be fp16, int8 or float8_e4m3fn, got {x.dtype}")
+        _row_scale("gemv_w4", "x_scale", x_scale, m)
+    act_c, out_c, _, _ = _tail_args("gemv_w4", out, n, m, bias, res1, res2, act)
+    _chk(_lib().dtas_gemv_w4(x.data_ptr(), _ptr(x_scale), w.data_ptr(), w_scale.data_ptr(), _ptr(w_zero), _ptr(bias),
+                             _ptr(res1), _ptr(res2), out.data_ptr(), m, n, k, k // groups, act_c, x_code, out_c, dev, st))
+    return out
+
+
+def gemm_nt_f8(x, w, x_scale, w_scale, out, bias=None, res1=None, res2=None, act=None):
+    """out[m, N] = act(x_scale[m] * w_scale[N] * (x[m, K] @ w[N, K]^T) + bias[N]) + res1 + res2 of float8_e4m3fn
+    operands with fp32 scales per row of x and per row of w (as quantize writes them); fp32 accumulation,
+    fp16 or fp32 `out`.  The tail, and an `out` that is a column slab of a wider buffer, are those of gemm_nt."""
+    dev_t = x.device
+    if dev_t.type != "cuda":
+        raise _abi.DtasError(_abi.EINVAL, f"gemm_f8: tensors must live on a CUDA device, got {dev_t}")
+    m, k = _rows_cols(x, "gemm_f8")
+    mo, n = _rows_cols(out, "gemm_f8")
+    if w.dim() != 2 or int(w.shape[1]) != k or int(w.shape[0]) != n or mo != m:
+        raise _abi.DtasError(_abi.EINVAL, f"gemm_f8: shapes x{tuple(x.shape)} w{tuple(w.shape)} out{tuple(out.shape)}")
+    if not (x.dtype == w.dtype == torch.float8_e4m3fn):
+        raise _abi.DtasError(_abi.EUNSUPPORTED, "gemm_f8: x and w must be float8_e4m3fn")
+    _row_scale("gemm_f8", "x_scale", x_scale, m)
+    _row_scale("gemm_f8", "w_scale", w_scale, n)
+    for t in (x, w, x_scale, w_scale):
+        if not t.is_contiguous():
+            raise _abi.DtasError(_abi.EINVAL, "gemm_f8: x, w and the scales must be contiguous")
+    if out.stride(-1) != 1:
+        raise _abi.DtasError(_abi.EINVAL, "gemm_f8: out must have unit stride in its last dim")
+    ldy = int(out.stride(-2)) if m > 1 else max(int(out.stride(-2)), n)
+    for t in (w, x_scale, w_scale, out, bias, res1, res2):
+        if t is not None and t.device != dev_t:
+            raise _abi.DtasError(_abi.EINVAL, "gemm_f8: tensors on different devices")
+    act_c, out_c, ldr, _ = _tail_args("gemm_f8", out, n, m, bias, res1, res2, act)
+    dev = dev_t.index if dev_t.index is not None else torch.cuda.current_device()
+    _chk(_lib().dtas_gemm_nt_f8(x.data_ptr(), w.data_ptr(), x_scale.data_ptr(), w_scale.data_ptr(), _ptr(bias), _ptr(res1),
+                                _ptr(res2), out.data_ptr(), m, n, k, ldy, ldr, act_c, out_c, dev, _raw_stream(dev)))
     return out
 
 

@@ -46,6 +46,7 @@ extern "C" {
 #define DTAS_F16  0
 #define DTAS_F32  1
 #define DTAS_I8   2
+#define DTAS_E4M3 3  /* 8-bit float with 4 exponent and 3 mantissa bits, largest value 448 */
 
 /* ---- elementwise class --------------------------------------------------
  * Replaces the generated `cast`, `add`, `copy` packed functions
@@ -118,6 +119,40 @@ int dtas_gemm_nt_fused(const void* x, const void* w, const void* bias, const voi
 int dtas_gemv_fused(const void* x, const void* w, const void* bias, const void* res1, const void* res2,
                     void* y, int64_t n, int64_t k, int act, int out_dtype, int dtype, int device, void* stream);
 
+/* ---- the low-bit path ------------------------------------------------------
+ * No counterpart in the reference.  What a layer with 8-bit or 4-bit weights calls in place of dtas_add,
+ * dtas_rms_norm, dtas_gemv and dtas_gemm_nt.
+ *
+ * dtas_add_rms_norm: h = x + res, y = h / sqrt(mean(h^2) + eps) * weight, row by row, in one launch.
+ *   x, res [m, n_cols] of in_dtype (DTAS_F16 or DTAS_F32); res may be NULL (h = x).  res_out, optional, receives
+ *   h in in_dtype and may be x or res itself; weight fp16 [n_cols].  The norm is taken of h before that
+ *   rounding.  y is out_dtype: DTAS_F16, or DTAS_I8 / DTAS_E4M3 with one fp32 scale per row in scale [m]:
+ *   scale = max|y| / Q, y = round(value / scale), Q = 127 or 448, ties to even.  A row of zeros gets scale 0
+ *   (y = 0); a row whose values hold an infinity or a NaN gets a NaN scale.  scale is not used for fp16.
+ * dtas_quantize: the same 8-bit form of the rows of x itself; also how a weight matrix [n, k] is brought to
+ *   8 bits with a scale per row for dtas_gemm_nt_f8.
+ * dtas_gemv_w4: y[m, n] = act(x . W^T + bias) + res1 + res2 for m <= DTAS_W4_MAX_ROWS rows, where
+ *   W[n, k] = w_scale[n, k / group] * (code - w_zero[n, k / group]).  w holds two 4-bit codes to a byte, [n, k / 2],
+ *   the even k in the low half; w_scale fp16 and w_zero uint8 [n, k / group]; w_zero NULL stands for 8 everywhere.
+ *   x is DTAS_F16 with x_scale NULL, or DTAS_I8 / DTAS_E4M3 with an fp32 scale per row.  k must be even and
+ *   a multiple of group.  Tail operands as in dtas_gemv_fused, with rows of n elements.  Groups and k that are
+ *   multiples of 32 with 16-byte aligned x and w take the fast kernel, everything else a scalar one.
+ * dtas_gemm_nt_f8: y = act(x_scale[m] w_scale[n] (x . w^T) + bias) + res1 + res2 of e4m3 operands x [m, k] and
+ *   w [n, k] with fp32 scales per row of each, on the tcgen05 tensor cores; ldy, ldr and the tail as in
+ *   dtas_gemm_nt_fused.  k a multiple of 16 and 16-byte aligned operands; else a scalar kernel.  Its
+ *   dispatch is that of dtas_gemm_nt for k / 2, overrides and measured table included.                   */
+#define DTAS_W4_MAX_ROWS 16
+int dtas_add_rms_norm(const void* x, const void* res, const void* weight, void* y, void* res_out, float* scale,
+                      int64_t m, int64_t n_cols, float eps, int in_dtype, int out_dtype, int device, void* stream);
+int dtas_quantize(const void* x, void* q, float* scale, int64_t m, int64_t n_cols, int in_dtype, int out_dtype,
+                  int device, void* stream);
+int dtas_gemv_w4(const void* x, const float* x_scale, const void* w, const void* w_scale, const void* w_zero,
+                 const void* bias, const void* res1, const void* res2, void* y, int64_t m, int64_t n, int64_t k,
+                 int64_t group, int act, int x_dtype, int out_dtype, int device, void* stream);
+int dtas_gemm_nt_f8(const void* x, const void* w, const float* x_scale, const float* w_scale, const void* bias,
+                    const void* res1, const void* res2, void* y, int64_t m, int64_t n, int64_t k, int64_t ldy,
+                    int64_t ldr, int act, int out_dtype, int device, void* stream);
+
 /* ---- GEMM without any allocation ------------------------------------------
  * No counterpart in the reference.  Same operation and operands as dtas_gemm_nt, for callers
  * that must not create device memory when they call: runtimes that gave the whole device to
@@ -153,7 +188,8 @@ int dtas_gemm_nt_static_scratch_plan(int64_t m, int64_t n, int64_t k, int split_
  * the generated `index = (n/256) > L ? L : n/256` statement
  * (python/dtas/engine/tuner.py:156-209) with the off-by-one at multiples of the
  * width removed: bucket = min((m-1)/256, last).  op is one of "cast", "add",
- * "copy", "rms_norm", "softmax", "layer_norm", "gemv", "gemm".  Returns -1 for
+ * "copy", "rms_norm", "softmax", "layer_norm", "gemv", "gemm", "add_rms_norm", "quantize", "gemv_w4",
+ * "gemm_f8".  Returns -1 for
  * an unknown op or m <= 0.
  * dtas_variant_of: writes the name of the kernel variant that the given call
  * shape would launch (e.g. "gemm_tc_bn256_s4_splitk1") into buf; returns DTAS_OK. */
