@@ -176,7 +176,7 @@ void row_quant_variant_name(const char* op, int64_t m, int64_t n_cols, char* buf
 
 int launch_gemv_w4(const void* x, const float* x_scale, const void* w, const void* w_scale, const void* w_zero,
                    const Epilogue& epi, void* y, int64_t m, int64_t n, int64_t k, int64_t group, int x_dtype,
-                   cudaStream_t st);
+                   const DeviceCtx* ctx, cudaStream_t st);
 
 int launch_gemv(const void* x, const void* w, const Epilogue& epi, void* y, int64_t n, int64_t k,
                 const DeviceCtx* ctx, cudaStream_t st);

@@ -360,7 +360,7 @@ int dtas_gemv_w4(const void* x, const float* x_scale, const void* w, const void*
   epi.ldr = n;
   epi.act = act;
   epi.out_f32 = out_dtype == DTAS_F32 ? 1 : 0;
-  return launch_gemv_w4(x, x_scale, w, w_scale, w_zero, epi, y, m, n, k, group, x_dtype, c.stream);
+  return launch_gemv_w4(x, x_scale, w, w_scale, w_zero, epi, y, m, n, k, group, x_dtype, c.ctx, c.stream);
 }
 
 int dtas_gemm_nt_f8(const void* x, const void* w, const float* x_scale, const float* w_scale, const void* bias,
