@@ -182,10 +182,12 @@ def w4_case(m, n, k, group, x_dtype=F16, zero=False, seed=0):
     z = 8.0 if c["w_zero"] is None else c["w_zero"].double()[..., None]
     w = ((c["codes"].double().view(n, groups, group) - z) * c["w_scale"].double()[..., None]).view(n, k)
     xs = c["x"].double() if c["x_scale"] is None else c["x"].double() * c["x_scale"].double()[:, None]
-    c["y"], c["abs"] = xs @ w.t(), xs.abs() @ w.abs().t()
-    # products are exact; sums of a group inside the MMAs (a truncated step of 2^-23 each), one fp32 rounding a group and
-    # warp, the scales: that many steps of 2^-22 of the sum of magnitudes, at most
-    c["slack"] = c["abs"] * ((max(group // 16, k // 32) + k // group + 24) * 2.0 ** -22)
+    c["y"] = xs @ w.t()
+    # codes (up to 15) and zero points times the group's sum of x are added up apart, so what is rounded is measured by 30
+    # times the scale times |x|; products are exact; sums of a group inside the MMAs (a truncated step of 2^-23 each), one
+    # fp32 rounding a group and warp, the scales: that many steps of 2^-23, at most
+    mag = xs.abs() @ (30 * c["w_scale"].double()[..., None].expand(n, groups, group).reshape(n, k)).t()
+    c["slack"] = mag * ((max(group // 16, k // 32) + k // group + 24) * 2.0 ** -23)
     return c
 
 
@@ -220,6 +222,23 @@ def test_gemv_w4_wide(cuda_device, m, n, k, group):
     again = torch.empty_like(out)
     w4_call(c, again)
     assert torch.equal(out, again)      # the same sums in the same order
+
+
+@pytest.mark.parametrize("zero", [False, True])
+@pytest.mark.parametrize("x_dtype", [F16, I8])
+@pytest.mark.parametrize("m,n,k,group", [(16, 4096, 11008, 128), (16, 9001, 20480, 64), (8, 5000, 16384, 32), (9, 9000, 4096, 128), (2, 300, 40960, 256)])
+def test_gemv_w4_with_k_shared_out(cuda_device, m, n, k, group, x_dtype, zero):
+    """Rows of x that do not fit one CTA's shared memory: K over the CTAs of a cluster, several tiles each, in one
+    batch and in several."""
+    c = w4_case(m, n, k, group, x_dtype, zero, seed=k)
+    out = torch.empty(m, n, dtype=F16, device="cuda")
+    bias = randn(n, seed=5).to(F16)
+    w4_call(c, out, bias=bias)
+    ops.poll_status()
+    assert_fp16_close(out, c["y"] + bias.double(), c["slack"])
+    again = torch.empty_like(out)
+    w4_call(c, again, bias=bias)
+    assert torch.equal(out, again)
 
 
 def gelu(v):
