@@ -17,6 +17,10 @@
 // consecutive elements, all loads in flight at once.  The threads per row are the row's chunks over CH,
 // rounded up to whole warps and not to a power of two, so that 11008 columns take 352 threads x 4 chunks
 // and none idles.  Bound: HBM; every element is read once and written once.
+// Rows of a length that is no multiple of eight start anywhere inside a 16-byte vector, but at the same place in
+// every operand (EDGE): chunks are cut where the flat index is a multiple of eight, and only the first and the last
+// of a row, which it shares with its neighbours, go element by element ([8192, 4097] to e4m3 143 us element by
+// element throughout).
 #include <cuda_fp8.h>
 
 #include "common.cuh"
@@ -125,6 +129,39 @@ __device__ __forceinline__ void store_q(OutT* p, const float* v) {
   }
 }
 
+// VEC weights as loaded.  They go through the read-only path: stores of the residual cannot alias them, so all of them are
+// under way with the rows instead of one behind each store.
+template <int VEC, bool EDGE>
+struct Weights {
+  static constexpr int kN = VEC == 8 ? 4 : VEC;
+  uint32_t r[kN];
+  __device__ __forceinline__ void load(const __half* p, int e, int n) {
+    const unsigned short* u = reinterpret_cast<const unsigned short*>(p);
+    if constexpr (VEC == 8 && !EDGE) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p + e));
+      r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w;
+    } else if constexpr (VEC == 8) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = e + 2 * i;
+        const uint32_t lo = j >= 0 && j < n ? __ldg(u + j) : 0u, hi = j + 1 >= 0 && j + 1 < n ? __ldg(u + j + 1) : 0u;
+        r[i] = lo | (hi << 16);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) r[i] = __ldg(u + e + i);
+    }
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (VEC == 8) {
+      const __half2 h = *reinterpret_cast<const __half2*>(&r[i >> 1]);
+      return i & 1 ? __high2float(h) : __low2float(h);
+    } else {
+      return __half2float(__ushort_as_half((unsigned short)r[i]));
+    }
+  }
+};
+
 // max that keeps a NaN, so that a row with one is not taken for a finite row
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -155,6 +192,35 @@ __device__ __forceinline__ void row_reduce(float& sum, float& top, float2* ex) {
   }
 }
 
+// A chunk of a row whose first element is e: whole, or (EDGE) the part of it that is the row's.
+template <int VEC, bool EDGE>
+__device__ __forceinline__ bool whole(int e, int n) {
+  return !EDGE || (e >= 0 && e + VEC <= n);
+}
+template <int VEC, bool EDGE, typename T>
+__device__ __forceinline__ void load_chunk(const T* row, int e, int n, float* v) {
+  if (whole<VEC, EDGE>(e, n)) {
+    load_vec<VEC>(row + e, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = e + i >= 0 && e + i < n ? to_f32(row[e + i]) : 0.f;
+  }
+}
+template <int VEC, bool EDGE, typename T>
+__device__ __forceinline__ void store_chunk(T* row, int e, int n, const float* v) {
+  if (whole<VEC, EDGE>(e, n)) {
+    if constexpr (sizeof(T) == 1) store_q<VEC>(row + e, v);
+    else store_vec<VEC>(row + e, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      if (e + i >= 0 && e + i < n) {
+        if constexpr (sizeof(T) == 1) store_q<1>(row + e + i, v + i);
+        else store_vec<1>(row + e + i, v + i);
+      }
+  }
+}
+
 // What an element is multiplied by on its way to 8 bits, and the row's scale.  A maximum so small that
 // Q / top would overflow goes through two steps (`pre` then `mul`); a row of zeros gets q = 0; a row that
 // holds an infinity or a NaN gets a NaN scale, and so stands for NaN whatever its q.
@@ -171,29 +237,38 @@ __device__ __forceinline__ float quant_scale(float top, float r, float q) {
   return top < INFINITY ? (top * r) / q : __int_as_float(0x7fc00000);
 }
 
-template <int OP, typename InT, typename OutT, int VEC, int CH>
+template <int OP, typename InT, typename OutT, int VEC, int CH, bool EDGE>
 __global__ void __launch_bounds__(max_threads(VEC, CH)) row_quant_kernel(const RowArgs a) {
   __shared__ float2 ex[kMaxThreads / 32];
   constexpr bool kNorm = OP == Q_NORM;
   constexpr bool k8 = sizeof(OutT) == 1;
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   const bool live = row < a.m;
-  const int n = (int)a.n_cols;
+  const int n = live ? (int)a.n_cols : 0;
   const int64_t off = (live ? row : 0) * a.n_cols;
+  const int lead = EDGE ? (int)(off & (VEC - 1)) : 0;      // elements of its first chunk that are not the row's
   const InT* x = static_cast<const InT*>(a.x) + off;
+  int at[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) at[c] = (c * blockDim.x + threadIdx.x) * VEC - lead;
 
   pdl_wait();
   pdl_launch_dependents();
   float v[CH][VEC];
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    const int e = (c * blockDim.x + threadIdx.x) * VEC;
-    if (live && e < n) {
-      load_vec<VEC>(x + e, v[c]);
+    if (at[c] < n) {
+      load_chunk<VEC, EDGE>(x, at[c], n, v[c]);
     } else {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) v[c][i] = 0.f;
     }
+  }
+  Weights<VEC, EDGE> wt[CH];
+  if constexpr (kNorm) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+      if (at[c] < n) wt[c].load(a.weight, at[c], n);
   }
   float sum = 0.f, top = 0.f;
   if constexpr (kNorm) {
@@ -201,10 +276,9 @@ __global__ void __launch_bounds__(max_threads(VEC, CH)) row_quant_kernel(const R
       const InT* res = static_cast<const InT*>(a.res) + off;
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
-        const int e = (c * blockDim.x + threadIdx.x) * VEC;
-        if (live && e < n) {
+        if (at[c] < n) {
           float t[VEC];
-          load_vec<VEC>(res + e, t);
+          load_chunk<VEC, EDGE>(res, at[c], n, t);
 #pragma unroll
           for (int i = 0; i < VEC; ++i) v[c][i] += t[i];
         }
@@ -214,14 +288,11 @@ __global__ void __launch_bounds__(max_threads(VEC, CH)) row_quant_kernel(const R
     for (int c = 0; c < CH; ++c) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) sum = fmaf(v[c][i], v[c][i], sum);
-      const int e = (c * blockDim.x + threadIdx.x) * VEC;
-      if (live && e < n) {
-        if (a.res_out != nullptr) store_vec<VEC>(static_cast<InT*>(a.res_out) + off + e, v[c]);
+      if (at[c] < n) {
+        if (a.res_out != nullptr) store_chunk<VEC, EDGE>(static_cast<InT*>(a.res_out) + off, at[c], n, v[c]);
         if constexpr (k8) {
-          float w[VEC];
-          load_vec<VEC>(a.weight + e, w);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) v[c][i] *= w[i];
+          for (int i = 0; i < VEC; ++i) v[c][i] *= wt[c].get(i);
         }
       }
     }
@@ -242,24 +313,21 @@ __global__ void __launch_bounds__(max_threads(VEC, CH)) row_quant_kernel(const R
     if (threadIdx.x == 0) a.scale[row] = quant_scale(top, r, OutTraits<OutT>::kQ);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int e = (c * blockDim.x + threadIdx.x) * VEC;
-      if (e < n) {
+      if (at[c] < n) {
         float q[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) q[i] = (v[c][i] * qm.pre) * qm.mul;
-        store_q<VEC>(y + e, q);
+        store_chunk<VEC, EDGE>(y, at[c], n, q);
       }
     }
   } else {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int e = (c * blockDim.x + threadIdx.x) * VEC;
-      if (e < n) {
-        float w[VEC];
-        load_vec<VEC>(a.weight + e, w);
+      if (at[c] < n) {
+        float o[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) w[i] = __fmul_rn(__fmul_rn(v[c][i], r), w[i]);
-        store_vec<VEC>(reinterpret_cast<__half*>(y) + e, w);
+        for (int i = 0; i < VEC; ++i) o[i] = __fmul_rn(__fmul_rn(v[c][i], r), wt[c].get(i));
+        store_chunk<VEC, EDGE>(reinterpret_cast<__half*>(y), at[c], n, o);
       }
     }
   }
@@ -314,27 +382,34 @@ __global__ void __launch_bounds__(kMaxThreads) row_quant_long_kernel(const RowAr
 
 // ---- dispatch ------------------------------------------------------------------
 struct RowPlan {
-  int vec;       // 8, or 1 where a row's length or an address rules out 16-byte vectors; 0: the long kernel
+  int vec;       // 8, or 1 where an address rules out 16-byte vectors; 0: the long kernel
   int ch;        // chunks per thread
   int tpr;       // threads per row
   int rows;      // rows per CTA
+  bool edge;     // rows that start inside a vector
 };
 
-inline RowPlan row_plan(int64_t m, int64_t n_cols, bool vec_ok) {
-  RowPlan p{0, 0, 0, 0};
-  p.vec = vec_ok ? 8 : 1;
-  const int64_t chunks = (n_cols + p.vec - 1) / p.vec;
-  const int64_t most = vec_ok ? 8 * max_threads(8, 8) : 16 * max_threads(1, 16);
+inline RowPlan row_plan(int64_t m, int64_t n_cols, bool aligned, bool norm) {
+  RowPlan p{0, 0, 0, 0, false};
+  p.vec = aligned ? 8 : 1;
+  p.edge = aligned && n_cols % 8 != 0;
+  const int64_t chunks = (n_cols + p.vec - 1) / p.vec + (p.edge ? 1 : 0);
+  const int64_t most = aligned ? 8 * max_threads(8, 8) : 16 * max_threads(1, 16);
   if (chunks > most) {
     p.vec = 0;
+    p.edge = false;
     p.tpr = kMaxThreads;
     p.rows = 1;
     return p;
   }
-  if (vec_ok) p.ch = m <= 592 && chunks <= kMaxThreads ? 1 : (chunks <= 64 ? 2 : (chunks <= 2048 ? 4 : 8));
-  else p.ch = chunks <= 256 * 4 ? 4 : 16;
+  if (!aligned) {
+    p.ch = chunks <= 256 * 4 ? 4 : 16;
+  } else {
+    p.ch = m <= 592 || norm ? 1 : (chunks <= 128 ? 2 : 4);
+    while (chunks > (int64_t)p.ch * max_threads(8, p.ch)) p.ch *= 2;
+  }
   p.tpr = (int)((chunks + p.ch - 1) / p.ch + 31) / 32 * 32;
-  p.rows = p.tpr >= 256 ? 1 : 256 / p.tpr;
+  p.rows = p.tpr >= 64 ? 1 : 64 / p.tpr;
   return p;
 }
 
@@ -347,13 +422,14 @@ int launch_typed(const RowPlan& p, const RowArgs& a, cudaStream_t st) {
     launch_kernel(row_quant_long_kernel<OP, InT, OutT>, (unsigned)grid, block, 0, st, a);
     return after_launch("row_quant_long_kernel");
   }
-#define DTAS_ROWQ_CASE(V, C)                                                                       \
-  if (p.vec == V && p.ch == C) {                                                                   \
-    launch_kernel(row_quant_kernel<OP, InT, OutT, V, C>, (unsigned)grid, block, 0, st, a);         \
+#define DTAS_ROWQ_CASE(V, C, E)                                                                    \
+  if (p.vec == V && p.ch == C && p.edge == E) {                                                    \
+    launch_kernel(row_quant_kernel<OP, InT, OutT, V, C, E>, (unsigned)grid, block, 0, st, a);      \
     return after_launch("row_quant_kernel");                                                       \
   }
-  DTAS_ROWQ_CASE(8, 1) DTAS_ROWQ_CASE(8, 2) DTAS_ROWQ_CASE(8, 4) DTAS_ROWQ_CASE(8, 8)
-  DTAS_ROWQ_CASE(1, 4) DTAS_ROWQ_CASE(1, 16)
+  DTAS_ROWQ_CASE(8, 1, false) DTAS_ROWQ_CASE(8, 2, false) DTAS_ROWQ_CASE(8, 4, false) DTAS_ROWQ_CASE(8, 8, false)
+  DTAS_ROWQ_CASE(8, 1, true) DTAS_ROWQ_CASE(8, 2, true) DTAS_ROWQ_CASE(8, 4, true) DTAS_ROWQ_CASE(8, 8, true)
+  DTAS_ROWQ_CASE(1, 4, false) DTAS_ROWQ_CASE(1, 16, false)
 #undef DTAS_ROWQ_CASE
   DTAS_FAIL(DTAS_EINVAL, "row op: no kernel for %d x %d", p.vec, p.ch);
 }
@@ -370,9 +446,10 @@ int launch_out(const RowPlan& p, const RowArgs& a, int out_dtype, cudaStream_t s
 
 template <int OP>
 int launch_in(const RowArgs& a, int in_dtype, int out_dtype, cudaStream_t st) {
-  bool vec_ok = a.n_cols % 8 == 0 && aligned16(a.x) && aligned16(a.res) && aligned16(a.weight) && aligned16(a.res_out);
-  vec_ok = vec_ok && (reinterpret_cast<uintptr_t>(a.y) & (out_dtype == DTAS_F16 ? 15 : 7)) == 0;
-  const RowPlan p = row_plan(a.m, a.n_cols, vec_ok);
+  // with rows that start inside a vector the weights are read one by one
+  bool aligned = aligned16(a.x) && aligned16(a.res) && aligned16(a.res_out) && (a.n_cols % 8 != 0 || aligned16(a.weight));
+  aligned = aligned && (reinterpret_cast<uintptr_t>(a.y) & (out_dtype == DTAS_F16 ? 15 : 7)) == 0;
+  const RowPlan p = row_plan(a.m, a.n_cols, aligned, OP == Q_NORM);
   if (in_dtype == DTAS_F16) return launch_out<OP, __half>(p, a, out_dtype, st);
   if (in_dtype == DTAS_F32) return launch_out<OP, float>(p, a, out_dtype, st);
   DTAS_FAIL(DTAS_EUNSUPPORTED, "row op: unsupported input dtype %d", in_dtype);
@@ -392,9 +469,9 @@ int launch_quantize(const void* x, void* q, float* scale, int64_t m, int64_t n_c
 }
 
 void row_quant_variant_name(const char* op, int64_t m, int64_t n_cols, char* buf, int len) {
-  const RowPlan p = row_plan(m, n_cols, n_cols % 8 == 0);
+  const RowPlan p = row_plan(m, n_cols, true, strcmp(op, "quantize") != 0);
   if (p.vec == 0) snprintf(buf, len, "%s_long_cta%d", op, p.tpr);
-  else snprintf(buf, len, "%s_vec%d_tpr%d_ch%d", op, p.vec, p.tpr, p.ch);
+  else snprintf(buf, len, "%s_vec%d%s_tpr%d_ch%d", op, p.vec, p.edge ? "_edge" : "", p.tpr, p.ch);
 }
 
 }  // namespace dtas

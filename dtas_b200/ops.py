@@ -21,7 +21,6 @@ def _lib():
     return _L
 
 _DTYPE_CODE = {torch.float16: _abi.F16, torch.float32: _abi.F32, torch.int8: _abi.I8}
-_LOW_CODE = {torch.int8: _abi.I8, torch.float8_e4m3fn: _abi.E4M3}
 
 
 def _chk(status):
@@ -274,9 +273,38 @@ def gemm_nt_scatter(x, w, out, peers, bias=None, multicast=0):
     return out
 
 
+# ---- the low-bit path ------------------------------------------------------------------------
+# These calls launch kernels of a few microseconds, and every attribute read of a tensor costs a tenth of one: a call
+# first asks, in one expression, whether everything is as it should be, and only otherwise goes through the checks that
+# say what is not (or that let it pass, as [m, H] beside [1, m, H]).
+_IN_CODE = {torch.float16: _abi.F16, torch.float32: _abi.F32}
+_NORM_OUT = {torch.float16: _abi.F16, torch.int8: _abi.I8, torch.float8_e4m3fn: _abi.E4M3}
+_LOW_CODE = {torch.int8: _abi.I8, torch.float8_e4m3fn: _abi.E4M3}
+_W4_IN = {torch.float16: _abi.F16, torch.int8: _abi.I8, torch.float8_e4m3fn: _abi.E4M3}
+
+
 def _row_scale(name, what, t, rows):
     if t is None or t.dtype != torch.float32 or t.numel() != rows:
         raise _abi.DtasError(_abi.EINVAL, f"{name}: {what} must be an fp32 vector of {rows} elements")
+
+
+def _check_add_rms_norm(x, res, weight, out, res_out, scale):
+    _check("add_rms_norm", *[t for t in (x, res, weight, out, res_out, scale) if t is not None])
+    m, h = _rows_cols(x, "add_rms_norm")
+    _same_shape("add_rms_norm", x, out)
+    for t in (res, res_out):
+        if t is not None:
+            _same_shape("add_rms_norm", x, t)
+            if t.dtype != x.dtype:
+                raise _abi.DtasError(_abi.EINVAL, "add_rms_norm: res and res_out must have x's dtype")
+    if x.dtype not in _IN_CODE:
+        raise _abi.DtasError(_abi.EUNSUPPORTED, f"add_rms_norm: x must be fp16 or fp32, got {x.dtype}")
+    if out.dtype not in _NORM_OUT:
+        raise _abi.DtasError(_abi.EUNSUPPORTED, f"add_rms_norm: out must be fp16, int8 or float8_e4m3fn, got {out.dtype}")
+    if weight.dtype != torch.float16 or weight.numel() != h:
+        raise _abi.DtasError(_abi.EINVAL, "add_rms_norm: weight must be fp16 [H]")
+    if out.dtype != torch.float16:
+        _row_scale("add_rms_norm", "scale", scale, m)
 
 
 def add_rms_norm(x, res, weight, out, res_out=None, scale=None, eps=1e-6):
@@ -286,42 +314,71 @@ def add_rms_norm(x, res, weight, out, res_out=None, scale=None, eps=1e-6):
     has x's dtype and may be x or res itself.  `out` is fp16, or int8 / float8_e4m3fn: then `scale`, fp32 [m],
     receives max|row| / Q (Q = 127 or 448) and out holds the row over its scale, rounded to even.  A row
     of zeros gets scale 0; a row with an infinity or a NaN gets a NaN scale."""
-    tensors = [t for t in (x, res, weight, out, res_out, scale) if t is not None]
-    dev, st = _check("add_rms_norm", *tensors)
-    m, h = _rows_cols(x, "add_rms_norm")
-    for t in (res, res_out):
-        if t is not None:
-            _same_shape("add_rms_norm", x, t)
-            if t.dtype != x.dtype:
-                raise _abi.DtasError(_abi.EINVAL, "add_rms_norm: res and res_out must have x's dtype")
-    _same_shape("add_rms_norm", x, out)
-    if weight.dtype != torch.float16 or weight.numel() != h:
-        raise _abi.DtasError(_abi.EINVAL, "add_rms_norm: weight must be fp16 [H]")
-    if out.dtype == torch.float16:
-        code, scale = _abi.F16, None
-    else:
-        code = _LOW_CODE.get(out.dtype)
-        if code is None:
-            raise _abi.DtasError(_abi.EUNSUPPORTED, f"add_rms_norm: out must be fp16, int8 or float8_e4m3fn, got {out.dtype}")
-        _row_scale("add_rms_norm", "scale", scale, m)
-    _chk(_lib().dtas_add_rms_norm(x.data_ptr(), _ptr(res), weight.data_ptr(), out.data_ptr(), _ptr(res_out), _ptr(scale),
-                                  m, h, float(eps), _code(x), code, dev, st))
+    dev, shape, dtype = x.get_device(), x.shape, x.dtype
+    code = _NORM_OUT.get(out.dtype)
+    if (dev < 0 or code is None or dtype not in _IN_CODE or len(shape) != 2 or out.shape != shape or weight.dtype != torch.float16
+            or weight.numel() != shape[1] or weight.get_device() != dev or out.get_device() != dev
+            or not (x.is_contiguous() and weight.is_contiguous() and out.is_contiguous())
+            or (res is not None and (res.shape != shape or res.dtype != dtype or res.get_device() != dev or not res.is_contiguous()))
+            or (res_out is not None and (res_out.shape != shape or res_out.dtype != dtype or res_out.get_device() != dev
+                                         or not res_out.is_contiguous()))
+            or ((scale is not None or code) and (scale is None or scale.dtype != torch.float32 or scale.numel() != shape[0]
+                                                 or scale.get_device() != dev or not scale.is_contiguous()))):
+        _check_add_rms_norm(x, res, weight, out, res_out, scale)
+    status = (_L or _lib()).dtas_add_rms_norm(
+        x.data_ptr(), None if res is None else res.data_ptr(), weight.data_ptr(), out.data_ptr(),
+        None if res_out is None else res_out.data_ptr(), None if scale is None else scale.data_ptr(),
+        shape[-2], shape[-1], float(eps), _IN_CODE[dtype], code, dev, _raw_stream(dev))
+    if status:
+        _abi.check(status)
     return out
+
+
+def _check_quantize(x, out, scale):
+    _check("quantize", x, out, scale)
+    _same_shape("quantize", x, out)
+    if x.dtype not in _IN_CODE:
+        raise _abi.DtasError(_abi.EUNSUPPORTED, f"quantize: x must be fp16 or fp32, got {x.dtype}")
+    if out.dtype not in _LOW_CODE:
+        raise _abi.DtasError(_abi.EUNSUPPORTED, f"quantize: out must be int8 or float8_e4m3fn, got {out.dtype}")
+    _row_scale("quantize", "scale", scale, _rows_cols(x, "quantize")[0])
 
 
 def quantize(x, out, scale):
     """Rows of x (fp16 or fp32) as int8 or float8_e4m3fn in `out` with one scale each in `scale` (fp32 [m]), as
     add_rms_norm writes them: for activations that no norm precedes, and for the weights of gemm_nt_f8 (a
     scale per output column)."""
-    dev, st = _check("quantize", x, out, scale)
-    _same_shape("quantize", x, out)
-    m, h = _rows_cols(x, "quantize")
+    dev, shape, dtype = x.get_device(), x.shape, x.dtype
     code = _LOW_CODE.get(out.dtype)
-    if code is None:
-        raise _abi.DtasError(_abi.EUNSUPPORTED, f"quantize: out must be int8 or float8_e4m3fn, got {out.dtype}")
-    _row_scale("quantize", "scale", scale, m)
-    _chk(_lib().dtas_quantize(x.data_ptr(), out.data_ptr(), scale.data_ptr(), m, h, _code(x), code, dev, st))
+    if (dev < 0 or code is None or dtype not in _IN_CODE or len(shape) != 2 or out.shape != shape or out.get_device() != dev
+            or scale.dtype != torch.float32 or scale.numel() != shape[0] or scale.get_device() != dev
+            or not (x.is_contiguous() and out.is_contiguous() and scale.is_contiguous())):
+        _check_quantize(x, out, scale)
+    status = (_L or _lib()).dtas_quantize(x.data_ptr(), out.data_ptr(), scale.data_ptr(), shape[-2], shape[-1], _IN_CODE[dtype],
+                                          code, dev, _raw_stream(dev))
+    if status:
+        _abi.check(status)
     return out
+
+
+def _check_gemv_w4(x, w, w_scale, out, w_zero, x_scale, bias, res1, res2, act):
+    _check("gemv_w4", *[t for t in (x, w, w_scale, out, w_zero, x_scale, bias, res1, res2) if t is not None])
+    m, k = _rows_cols(x, "gemv_w4")
+    mo, n = _rows_cols(out, "gemv_w4")
+    if w.dtype != torch.uint8 or w.dim() != 2 or mo != m or tuple(w.shape) != (n, k // 2) or k % 2:
+        raise _abi.DtasError(_abi.EINVAL, f"gemv_w4: shapes x{tuple(x.shape)} w{tuple(w.shape)} out{tuple(out.shape)}; w is uint8 [N, K / 2]")
+    groups = int(w_scale.shape[1]) if w_scale.dim() == 2 else 0
+    if w_scale.dtype != torch.float16 or groups < 1 or int(w_scale.shape[0]) != n or k % groups:
+        raise _abi.DtasError(_abi.EINVAL, f"gemv_w4: w_scale must be fp16 [N, groups] with groups a divisor of K, got {tuple(w_scale.shape)}")
+    if w_zero is not None and (w_zero.dtype != torch.uint8 or w_zero.shape != w_scale.shape):
+        raise _abi.DtasError(_abi.EINVAL, "gemv_w4: w_zero must be uint8 with w_scale's shape")
+    if x.dtype not in _W4_IN:
+        raise _abi.DtasError(_abi.EUNSUPPORTED, f"gemv_w4: x must be fp16, int8 or float8_e4m3fn, got {x.dtype}")
+    if x.dtype != torch.float16:
+        _row_scale("gemv_w4", "x_scale", x_scale, m)
+    elif x_scale is not None:
+        raise _abi.DtasError(_abi.EINVAL, "gemv_w4: x_scale belongs to an x of 8 bits")
+    _tail_args("gemv_w4", out, n, m, bias, res1, res2, act)
 
 
 def gemv_w4(x, w, w_scale, out, w_zero=None, x_scale=None, bias=None, res1=None, res2=None, act=None):
@@ -332,36 +389,35 @@ def gemv_w4(x, w, w_scale, out, w_zero=None, x_scale=None, bias=None, res1=None,
     what G is; `w_zero` uint8 of the same shape, 8 everywhere when None (dtas_b200.weights.quantize_w4
     makes all three).  x is fp16, or int8 / float8_e4m3fn with x_scale fp32 [m], as add_rms_norm and
     quantize write them.  out is fp16 or fp32 (the fp16 result widened); the tail is that of gemv."""
-    tensors = [t for t in (x, w, w_scale, out, w_zero, x_scale, bias, res1, res2) if t is not None]
-    dev, st = _check("gemv_w4", *tensors)
-    m, k = _rows_cols(x, "gemv_w4")
-    mo, n = _rows_cols(out, "gemv_w4")
-    if w.dtype != torch.uint8 or w.dim() != 2 or mo != m or tuple(w.shape) != (n, k // 2) or k % 2:
-        raise _abi.DtasError(_abi.EINVAL, f"gemv_w4: shapes x{tuple(x.shape)} w{tuple(w.shape)} out{tuple(out.shape)}; w is uint8 [N, K / 2]")
-    groups = int(w_scale.shape[1]) if w_scale.dim() == 2 else 0
-    if w_scale.dtype != torch.float16 or groups < 1 or int(w_scale.shape[0]) != n or k % groups:
-        raise _abi.DtasError(_abi.EINVAL, f"gemv_w4: w_scale must be fp16 [N, groups] with groups a divisor of K, got {tuple(w_scale.shape)}")
-    if w_zero is not None and (w_zero.dtype != torch.uint8 or w_zero.shape != w_scale.shape):
-        raise _abi.DtasError(_abi.EINVAL, "gemv_w4: w_zero must be uint8 with w_scale's shape")
-    if x.dtype == torch.float16:
-        x_code = _abi.F16
-        if x_scale is not None:
-            raise _abi.DtasError(_abi.EINVAL, "gemv_w4: x_scale belongs to an x of 8 bits")
-    else:
-        x_code = _LOW_CODE.get(x.dtype)
-        if x_code is None:
-            raise _abi.DtasError(_abi.EUNSUPPORTED, f"gemv_w4: x must be fp16, int8 or float8_e4m3fn, got {x.dtype}")
-        _row_scale("gemv_w4", "x_scale", x_scale, m)
-    act_c, out_c, _, _ = _tail_args("gemv_w4", out, n, m, bias, res1, res2, act)
-    _chk(_lib().dtas_gemv_w4(x.data_ptr(), _ptr(x_scale), w.data_ptr(), w_scale.data_ptr(), _ptr(w_zero), _ptr(bias),
-                             _ptr(res1), _ptr(res2), out.data_ptr(), m, n, k, k // groups, act_c, x_code, out_c, dev, st))
+    dev, xs, os, gs, dtype = x.get_device(), x.shape, out.shape, w_scale.shape, x.dtype
+    code = _W4_IN.get(dtype)
+    if (dev < 0 or code is None or len(xs) != 2 or len(os) != 2 or len(gs) != 2 or xs[0] != os[0] or os[1] != gs[0]
+            or w.shape != (gs[0], xs[1] >> 1) or xs[1] & 1 or gs[1] < 1 or xs[1] % gs[1] or w.dtype != torch.uint8
+            or w_scale.dtype != torch.float16 or w.get_device() != dev or w_scale.get_device() != dev or out.get_device() != dev
+            or not (x.is_contiguous() and w.is_contiguous() and w_scale.is_contiguous() and out.is_contiguous())
+            or (x_scale is None) != (code == _abi.F16)
+            or (x_scale is not None and (x_scale.dtype != torch.float32 or x_scale.numel() != xs[0] or x_scale.get_device() != dev
+                                         or not x_scale.is_contiguous()))
+            or (w_zero is not None and (w_zero.dtype != torch.uint8 or w_zero.shape != gs or w_zero.get_device() != dev
+                                        or not w_zero.is_contiguous()))
+            or act not in _ACTS or out.dtype not in _IN_CODE
+            or (bias is not None and (bias.dtype != torch.float16 or bias.numel() != os[1] or bias.get_device() != dev or not bias.is_contiguous()))
+            or (res1 is not None and (res1.dtype != torch.float16 or res1.shape != os or res1.get_device() != dev or not res1.is_contiguous()))
+            or (res2 is not None and (res1 is None or res2.dtype != torch.float16 or res2.shape != os or res2.get_device() != dev
+                                      or not res2.is_contiguous()))):
+        _check_gemv_w4(x, w, w_scale, out, w_zero, x_scale, bias, res1, res2, act)
+    status = (_L or _lib()).dtas_gemv_w4(
+        x.data_ptr(), None if x_scale is None else x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
+        None if w_zero is None else w_zero.data_ptr(), None if bias is None else bias.data_ptr(),
+        None if res1 is None else res1.data_ptr(), None if res2 is None else res2.data_ptr(), out.data_ptr(),
+        xs[-2], os[-1], xs[-1], xs[-1] // gs[1], _ACTS[act], code, _IN_CODE[out.dtype], dev, _raw_stream(dev))
+    if status:
+        _abi.check(status)
     return out
 
 
-def gemm_nt_f8(x, w, x_scale, w_scale, out, bias=None, res1=None, res2=None, act=None):
-    """out[m, N] = act(x_scale[m] * w_scale[N] * (x[m, K] @ w[N, K]^T) + bias[N]) + res1 + res2 of float8_e4m3fn
-    operands with fp32 scales per row of x and per row of w (as quantize writes them); fp32 accumulation,
-    fp16 or fp32 `out`.  The tail, and an `out` that is a column slab of a wider buffer, are those of gemm_nt."""
+def _check_gemm_nt_f8(x, w, x_scale, w_scale, out, bias, res1, res2, act):
+    """-> ldr"""
     dev_t = x.device
     if dev_t.type != "cuda":
         raise _abi.DtasError(_abi.EINVAL, f"gemm_f8: tensors must live on a CUDA device, got {dev_t}")
@@ -378,14 +434,38 @@ def gemm_nt_f8(x, w, x_scale, w_scale, out, bias=None, res1=None, res2=None, act
             raise _abi.DtasError(_abi.EINVAL, "gemm_f8: x, w and the scales must be contiguous")
     if out.stride(-1) != 1:
         raise _abi.DtasError(_abi.EINVAL, "gemm_f8: out must have unit stride in its last dim")
-    ldy = int(out.stride(-2)) if m > 1 else max(int(out.stride(-2)), n)
     for t in (w, x_scale, w_scale, out, bias, res1, res2):
         if t is not None and t.device != dev_t:
             raise _abi.DtasError(_abi.EINVAL, "gemm_f8: tensors on different devices")
-    act_c, out_c, ldr, _ = _tail_args("gemm_f8", out, n, m, bias, res1, res2, act)
-    dev = dev_t.index if dev_t.index is not None else torch.cuda.current_device()
-    _chk(_lib().dtas_gemm_nt_f8(x.data_ptr(), w.data_ptr(), x_scale.data_ptr(), w_scale.data_ptr(), _ptr(bias), _ptr(res1),
-                                _ptr(res2), out.data_ptr(), m, n, k, ldy, ldr, act_c, out_c, dev, _raw_stream(dev)))
+    return _tail_args("gemm_f8", out, n, m, bias, res1, res2, act)[2]
+
+
+def gemm_nt_f8(x, w, x_scale, w_scale, out, bias=None, res1=None, res2=None, act=None):
+    """out[m, N] = act(x_scale[m] * w_scale[N] * (x[m, K] @ w[N, K]^T) + bias[N]) + res1 + res2 of float8_e4m3fn
+    operands with fp32 scales per row of x and per row of w (as quantize writes them); fp32 accumulation,
+    fp16 or fp32 `out`.  The tail, and an `out` that is a column slab of a wider buffer, are those of gemm_nt."""
+    dev, xs, ws, os, ldr = x.get_device(), x.shape, w.shape, out.shape, 0
+    f8 = torch.float8_e4m3fn
+    if (dev < 0 or len(xs) != 2 or len(ws) != 2 or len(os) != 2 or xs[1] != ws[1] or os != (xs[0], ws[0])
+            or x.dtype != f8 or w.dtype != f8 or x_scale.dtype != torch.float32 or w_scale.dtype != torch.float32
+            or x_scale.numel() != xs[0] or w_scale.numel() != ws[0] or w.get_device() != dev or x_scale.get_device() != dev
+            or w_scale.get_device() != dev or out.get_device() != dev
+            or not (x.is_contiguous() and w.is_contiguous() and x_scale.is_contiguous() and w_scale.is_contiguous() and out.is_contiguous())
+            or act not in _ACTS or out.dtype not in _IN_CODE
+            or (bias is not None and (bias.dtype != torch.float16 or bias.numel() != os[1] or bias.get_device() != dev or not bias.is_contiguous()))
+            or (res1 is not None and (res1.dtype != torch.float16 or res1.shape != os or res1.get_device() != dev or not res1.is_contiguous()))
+            or (res2 is not None and (res1 is None or res2.dtype != torch.float16 or res2.shape != os or res2.get_device() != dev
+                                      or not res2.is_contiguous()))):
+        ldr = _check_gemm_nt_f8(x, w, x_scale, w_scale, out, bias, res1, res2, act)
+    m, n = xs[-2], os[-1]
+    ldr = ldr or n
+    ldy = n if m == 1 or out.is_contiguous() else out.stride(-2)
+    status = (_L or _lib()).dtas_gemm_nt_f8(
+        x.data_ptr(), w.data_ptr(), x_scale.data_ptr(), w_scale.data_ptr(), None if bias is None else bias.data_ptr(),
+        None if res1 is None else res1.data_ptr(), None if res2 is None else res2.data_ptr(), out.data_ptr(),
+        m, n, xs[-1], ldy, ldr, _ACTS[act], _IN_CODE[out.dtype], dev, _raw_stream(dev))
+    if status:
+        _abi.check(status)
     return out
 
 
