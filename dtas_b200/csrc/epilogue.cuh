@@ -105,7 +105,6 @@ __device__ __forceinline__ float epi_tail(const Epilogue& e, float t, int64_t ro
 }
 // Value of one output element from its fp32 dot product.
 __device__ __forceinline__ float epi_value(const Epilogue& e, float acc, int64_t row, int col) {
-  if (e.sx != nullptr) acc = acc * e.sx[row] * e.sw[col];
   if (e.bias != nullptr) acc += __half2float(e.bias[col]);
   return epi_tail(e, acc, row, col);
 }
@@ -117,9 +116,9 @@ __device__ __forceinline__ void epi_store(const Epilogue& e, void* y, int64_t ld
 }
 
 // Scales of 8-bit operands and the bias on COUNT consecutive rows of one output column, in place.
-template <int COUNT>
+template <bool F8, int COUNT>
 __device__ __forceinline__ void epi_scale_bias_column(const Epilogue& e, int row0, int m, int col, float bias, float* v) {
-  if (e.sx != nullptr) {
+  if constexpr (F8) {
     const float sw = e.sw[col];
 #pragma unroll
     for (int j = 0; j < COUNT; ++j) v[j] = v[j] * (row0 + j < m ? e.sx[row0 + j] : 0.f) * sw;
@@ -232,7 +231,7 @@ __device__ __forceinline__ void epi_add_res32(const __half* res, int64_t off, in
 // True when the tail is nothing but an optional bias and an fp16 store: the path every plain GEMM
 // takes, kept free of the machinery below.
 __device__ __forceinline__ bool epi_is_plain(const Epilogue& e) {
-  return e.res1 == nullptr && e.act == DTAS_ACT_NONE && !e.out_f32 && e.sx == nullptr;
+  return e.res1 == nullptr && e.act == DTAS_ACT_NONE && !e.out_f32;
 }
 // The plain tail for 32 consecutive columns of one row, from the raw accumulator words.
 __device__ __forceinline__ void epi_store_row32_plain(const __half* bias, __half* yrow, int vec_store, int col0, int n,
@@ -291,12 +290,34 @@ __device__ __forceinline__ void epi_scale_row32(const Epilogue& e, int64_t row, 
   }
 }
 
+// Scales of 8-bit operands and the bias on 32 columns of one row, the columns' part from shared memory.
+__device__ __forceinline__ void epi_scale_bias_row32(const Epilogue& e, float sx, const float* sw, const __half* bias, float* acc32) {
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const float4 v = reinterpret_cast<const float4*>(sw)[q];
+    acc32[4 * q] = acc32[4 * q] * sx * v.x;
+    acc32[4 * q + 1] = acc32[4 * q + 1] * sx * v.y;
+    acc32[4 * q + 2] = acc32[4 * q + 2] * sx * v.z;
+    acc32[4 * q + 3] = acc32[4 * q + 3] * sx * v.w;
+  }
+  if (e.bias != nullptr) {
+    uint4 v[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = reinterpret_cast<const uint4*>(bias)[q];
+    epi_add_vec32(v, acc32);
+  }
+}
+
 // The arithmetic of the tail on 32 consecutive columns of one row, in place: scales of 8-bit operands, bias,
-// activation, residuals.  `pre`, when given, holds the residual values of this chunk fetched earlier.
+// activation, residuals.  `pre`, when given, holds the residual values of this chunk fetched earlier; `scaled`:
+// scales and bias have been applied (epi_scale_bias_row32).
+template <bool F8>
 __device__ __forceinline__ void epi_apply_row32(const Epilogue& e, int64_t row, int col0, int n, float* acc32,
-                                                const ResChunk* pre = nullptr) {
-  if (e.sx != nullptr) epi_scale_row32(e, row, col0, n, acc32);
-  if (e.bias != nullptr) epi_add_bias32(e.bias, col0, n, acc32);
+                                                const ResChunk* pre = nullptr, bool scaled = false) {
+  if (!scaled) {
+    if constexpr (F8) epi_scale_row32(e, row, col0, n, acc32);
+    if (e.bias != nullptr) epi_add_bias32(e.bias, col0, n, acc32);
+  }
   if (e.act == DTAS_ACT_GELU) {
 #pragma unroll
     for (int g = 0; g < 32; g += 8) gelu_erf_n<8>(acc32 + g);   // groups of 4 time the same, of 16 slower
@@ -356,14 +377,31 @@ __device__ __forceinline__ void epi_store_staged_block(const uint4* stage, int l
   }
 }
 
+// The same block element by element, for rows of Y that are not aligned and for its right edge: a store instruction
+// still writes 32 consecutive elements of one row.
+template <int CPR>
+__device__ __forceinline__ void epi_store_staged_elements(const uint4* stage, int lane, int64_t row_base, int m, void* y,
+                                                          int64_t ldy, int col0, int n) {
+  const __half* s = reinterpret_cast<const __half*>(stage);
+  const int rows = (int)(m - row_base < 32 ? m - row_base : 32), cols = n - col0 < 8 * CPR ? n - col0 : 8 * CPR;
+#pragma unroll 4
+  for (int rl = 0; rl < rows; ++rl) {
+    __half* to = static_cast<__half*>(y) + (row_base + rl) * ldy + col0;
+#pragma unroll
+    for (int j = lane; j < 8 * CPR; j += 32)
+      if (j < cols) to[j] = s[(rl * CPR + ((j >> 3) ^ (rl & 7))) * 8 + (j & 7)];
+  }
+}
+
 // Finishes 32 consecutive output columns col0 .. col0+31 of one row held in acc32 (fp32 dot
 // products) and stores them.  vec_store: 16-byte stores into Y rows are aligned.  `pre`, when
 // given, holds the residual values of this chunk fetched earlier (epi_prefetch_res32).
+template <bool F8>
 __device__ __forceinline__ void epi_store_row32(const Epilogue& e, void* y, int64_t ldy, int vec_store, int64_t row,
                                                 int col0, int n, float* acc32, const ResChunk* pre = nullptr,
-                                                const PeerOut* peers = nullptr) {
+                                                const PeerOut* peers = nullptr, bool scaled = false) {
   const int n_peers = peers != nullptr ? peers->n : 0;
-  epi_apply_row32(e, row, col0, n, acc32, pre);
+  epi_apply_row32<F8>(e, row, col0, n, acc32, pre, scaled);
   const bool full = vec_store && col0 + 32 <= n;
   if (!e.out_f32) {
     __half* yrow = static_cast<__half*>(y) + row * ldy;

@@ -37,7 +37,7 @@
 // m >= ~1024, HBM (W stream) for small m.
 //
 // The same kernels compute the product of e4m3 operands with a scale per row of X and per row of W
-// (dtas_gemm_nt_f8; GemmArgs::f8): the issuing thread uses the f8f6f4 kind of the instruction, which takes
+// (dtas_gemm_nt_f8; F8): the issuing thread uses the f8f6f4 kind of the instruction, which takes
 // 32 elements where the fp16 kind takes 16, and the epilogue starts with the scales.
 #include <cuda.h>
 #include <cuda_fp8.h>
@@ -172,14 +172,12 @@ __device__ __forceinline__ void umma(uint32_t d_tmem, uint64_t a_desc, uint64_t 
   }
 }
 // The MMAs of one k-block (one 128-byte swizzle row of both operands).
-__device__ __forceinline__ void umma_kblock(int f8, uint32_t d_tmem, uint64_t da, uint64_t db, uint32_t idesc, bool first) {
-  // advancing 16 fp16 or 32 e4m3 along K inside the swizzle row = +32 bytes = +2 in the address field
-  if (f8) {
+template <bool F8>
+__device__ __forceinline__ void umma_kblock(uint32_t d_tmem, uint64_t da, uint64_t db, uint32_t idesc, bool first) {
 #pragma unroll
-    for (int kk = 0; kk < BK / UMMA_K; ++kk) umma<true>(d_tmem, da + 2u * kk, db + 2u * kk, idesc, (!first || kk > 0) ? 1u : 0u);
-  } else {
-#pragma unroll
-    for (int kk = 0; kk < BK / UMMA_K; ++kk) umma<false>(d_tmem, da + 2u * kk, db + 2u * kk, idesc, (!first || kk > 0) ? 1u : 0u);
+  for (int kk = 0; kk < BK / UMMA_K; ++kk) {
+    // advancing 16 fp16 or 32 e4m3 along K inside the swizzle row = +32 bytes = +2 in the address field
+    umma<F8>(d_tmem, da + 2u * kk, db + 2u * kk, idesc, (!first || kk > 0) ? 1u : 0u);
   }
 }
 // Arrives on the mbarrier once every tcgen05.mma issued so far by this thread has retired.
@@ -249,7 +247,6 @@ struct GemmArgs {
   int sk_first = 0;   // two-CTA kernel, stream-K: first tile of the region that is cut into runs of units
   int slots_cap = 0;  // partial-tile slots reserved per output tile in the workspace
   PeerOut peers;      // two-CTA kernel: further buffers that receive every stored vector of Y
-  int f8 = 0;         // 1: X and W are e4m3, two elements to a 16-bit word of k (epi.sx / epi.sw scale the result)
 };
 
 template <int BN>
@@ -329,7 +326,7 @@ struct TileIter {
   }
 };
 
-template <int BN>
+template <int BN, bool F8>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     gemm_f16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_x,
                             const __grid_constant__ CUtensorMap tmap_w, const GemmArgs a) {
@@ -424,7 +421,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           const uint32_t sa = base + stage * C::kStageBytes;
           const uint64_t da = make_kmajor_sw128_desc(sa);
           const uint64_t db = make_kmajor_sw128_desc(sa + C::kABytes);
-          umma_kblock(a.f8, d_tmem, da, db, idesc, kb == kb0);
+          umma_kblock<F8>(d_tmem, da, db, idesc, kb == kb0);
           umma_commit(empty_bar(stage));   // stage reusable once these MMAs have read it
           if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
         }
@@ -453,7 +450,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       const int col_base = nt * BN;
 
       if (n_parts == 1) {
-        if (epi_is_plain(a.epi)) {
+        if (!F8 && epi_is_plain(a.epi)) {
           __half* yrow = static_cast<__half*>(a.y) + (int64_t)row * a.ldy;
           // blocks of 8 * kStoreCpr columns go through shared memory and leave as whole rows of 128 or 256
           // contiguous bytes (see epi_store_staged_block); ragged edges and unaligned Y from the registers
@@ -509,7 +506,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             float f[32];
 #pragma unroll
             for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(r[j]);
-            epi_store_row32(a.epi, a.y, a.ldy, a.vec_store, row, col0, a.n, f,
+            epi_store_row32<F8>(a.epi, a.y, a.ldy, a.vec_store, row, col0, a.n, f,
                             epi_can_prefetch(a.epi, col0, a.n) ? &r_now : nullptr);
           }
         }
@@ -602,7 +599,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                   acc[4 * q] += v1[q].x; acc[4 * q + 1] += v1[q].y; acc[4 * q + 2] += v1[q].z; acc[4 * q + 3] += v1[q].w;
                 }
               }
-              epi_store_row32(a.epi, a.y, a.ldy, a.vec_store, row, col0, a.n, acc);
+              epi_store_row32<F8>(a.epi, a.y, a.ldy, a.vec_store, row, col0, a.n, acc);
             }
           }
         }
@@ -707,7 +704,7 @@ struct SwapIter {
 };
 
 // a.n_tiles counts 128-column tiles of Y (128-row tiles of W); a.m_tiles is 1.
-template <int MN>
+template <int MN, bool F8>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     gemm_f16_tcgen05_swap_kernel(const __grid_constant__ CUtensorMap tmap_w,
                                  const __grid_constant__ CUtensorMap tmap_x, const GemmArgs a) {
@@ -797,7 +794,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           const uint32_t sa = base + stage * C::kStageBytes;
           const uint64_t da = make_kmajor_sw128_desc(sa);                // W rows: the M side
           const uint64_t db = make_kmajor_sw128_desc(sa + C::kWBytes);   // X rows: the N side
-          umma_kblock(a.f8, d_tmem, da, db, idesc, kb == kb0);
+          umma_kblock<F8>(d_tmem, da, db, idesc, kb == kb0);
           umma_commit(empty_bar(stage));
           if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
         }
@@ -836,7 +833,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             float f[kChunk];
 #pragma unroll
             for (int j = 0; j < kChunk; ++j) f[j] = __uint_as_float(r[j]);
-            epi_scale_bias_column<kChunk>(a.epi, c * kChunk, a.m, col, bias, f);
+            epi_scale_bias_column<F8, kChunk>(a.epi, c * kChunk, a.m, col, bias, f);
             epi_store_column<kChunk>(a.epi, a.y, a.ldy, c * kChunk, a.m, col, f);
           }
         }
@@ -920,7 +917,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 o[4 * j] = sum4[j].x; o[4 * j + 1] = sum4[j].y;
                 o[4 * j + 2] = sum4[j].z; o[4 * j + 3] = sum4[j].w;
               }
-              epi_scale_bias_column<4 * G>(a.epi, g0 * 4, a.m, col, bias, o);
+              epi_scale_bias_column<F8, 4 * G>(a.epi, g0 * 4, a.m, col, bias, o);
               epi_store_column<4 * G>(a.epi, a.y, a.ldy, g0 * 4, a.m, col, o);
             }
           }
@@ -1014,14 +1011,10 @@ __device__ __forceinline__ void umma_pair(uint32_t d_tmem, uint64_t a_desc, uint
         : "memory");
   }
 }
-__device__ __forceinline__ void umma_kblock_pair(int f8, uint32_t d_tmem, uint64_t da, uint64_t db, uint32_t idesc, bool first) {
-  if (f8) {
+template <bool F8>
+__device__ __forceinline__ void umma_kblock_pair(uint32_t d_tmem, uint64_t da, uint64_t db, uint32_t idesc, bool first) {
 #pragma unroll
-    for (int kk = 0; kk < BK / UMMA_K; ++kk) umma_pair<true>(d_tmem, da + 2u * kk, db + 2u * kk, idesc, (!first || kk > 0) ? 1u : 0u);
-  } else {
-#pragma unroll
-    for (int kk = 0; kk < BK / UMMA_K; ++kk) umma_pair<false>(d_tmem, da + 2u * kk, db + 2u * kk, idesc, (!first || kk > 0) ? 1u : 0u);
-  }
+  for (int kk = 0; kk < BK / UMMA_K; ++kk) umma_pair<F8>(d_tmem, da + 2u * kk, db + 2u * kk, idesc, (!first || kk > 0) ? 1u : 0u);
 }
 // Arrives on the barrier at this offset in every CTA of `cta_mask` once the MMAs issued so far retire.
 __device__ __forceinline__ void umma_commit_pair(uint32_t bar, uint16_t cta_mask) {
@@ -1053,8 +1046,9 @@ constexpr int kPairStages = DTAS_PAIR_STAGED_STORE ? 6 : 7;
 constexpr int kPairStoreStage = DTAS_PAIR_STAGED_STORE ? 4 * 32 * 256 : 0;
 constexpr int kPairTmemCols = 2 * kPairBN;
 constexpr int kPairBarBytes = (2 * kPairStages + 4) * 8 + 16;
+constexpr int kPairColBytes = kPairBN * (4 + 2);   // e4m3 operands: scales and bias of a tile's columns
 constexpr int kPairSmemBytes = 1024 + kPairStages * kPairStageBytes + kPairStoreStage + kPairBarBytes;
-static_assert(kPairSmemBytes <= 227 * 1024, "smem");
+static_assert(kPairSmemBytes + kPairColBytes <= 227 * 1024, "smem");
 constexpr int kPairGroupM = 16;              // 256-row tiles per rasterisation band (8: W re-read twice as often, 1-3 % slower; 32: 5-8 % slower)
 constexpr int ERR_PAIR_TAIL = 0x105;
 
@@ -1131,12 +1125,29 @@ __device__ __forceinline__ void epilogue_bar_sync_n(int threads) {
   asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");
 }
 
+// The same, and whether `ok` holds for all of them.
+__device__ __forceinline__ bool epilogue_bar_and_n(int threads, bool ok) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.and.pred q, 1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t"
+      "}"
+      : "=r"(all)
+      : "r"((uint32_t)ok), "r"(threads)
+      : "memory");
+  return all != 0;
+}
+
 constexpr int kPairMaxThreads = 32 * (2 + 8);   // producer, MMA issuer and up to eight epilogue warps
 
 // Launched with four epilogue warps (192 threads), or with eight (320 threads) when the epilogue has an
 // activation or residuals to work through: of the two warps that share a quarter of the tensor-memory
 // lanes one then finishes columns 0..127 of the tile and the other columns 128..255, so the tail of a
 // 256 x 256 tile is spread over twice the issue slots and hides behind a shorter main loop.
+template <bool F8>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairMaxThreads, 1)
     gemm_f16_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_x,
                                  const __grid_constant__ CUtensorMap tmap_w, const GemmArgs a) {
@@ -1153,6 +1164,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairMaxThreads, 1)
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(
       gen_base + kPairStages * kPairStageBytes + kPairStoreStage + 8 * (2 * kPairStages + 4));
   volatile uint32_t* last_flag_ptr = tmem_slot_ptr + 1;
+  float* col_scale = reinterpret_cast<float*>(gen_base + kPairStages * kPairStageBytes + kPairStoreStage + kPairBarBytes);
+  __half* col_bias = reinterpret_cast<__half*>(col_scale + kPairBN);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();          // 0 = leader
@@ -1239,7 +1252,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairMaxThreads, 1)
           const uint32_t sa = base + stage * kPairStageBytes;
           const uint64_t da = make_kmajor_sw128_desc(sa);
           const uint64_t db = make_kmajor_sw128_desc(sa + kPairHalfBytes);
-          umma_kblock_pair(a.f8, d_tmem, da, db, idesc, kb == sg.kb0);
+          umma_kblock_pair<F8>(d_tmem, da, db, idesc, kb == sg.kb0);
           umma_commit_pair(empty_bar(stage), 0x3);
           if (++stage == kPairStages) { stage = 0; phase ^= 1u; }
         }
@@ -1263,7 +1276,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairMaxThreads, 1)
       const int mt = sg.mt, nt = sg.nt;
       const int acc = iter & 1;
       const uint32_t acc_phase = (uint32_t)(iter >> 1) & 1u;
-      if (!mbar_wait(tfull_bar(acc), acc_phase, a.status, ERR_EPILOGUE)) { ok = false; break; }
+      float row_scale = 0.f, my_scale[2] = {0.f, 0.f};
+      __half my_bias[2] = {__half(0.f), __half(0.f)};
+      if constexpr (F8) {
+        // The main loop of an e4m3 tile is half as long as an fp16 tile's, too short to hide a trip to L2 for every 32
+        // columns' scales and bias behind it: a thread fetches its columns' (one of eight warps, two of four) while
+        // the tile is computed, and they wait in shared memory for the arithmetic.
+        const int r = mt * 2 * BM + (int)rank * BM + quarter * 32 + lane;
+        if (r < a.m) row_scale = a.epi.sx[r];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int c = epi_tid + e * n_epi_threads, col = nt * kPairBN + c;
+          if (c < kPairBN && col < a.n) {
+            my_scale[e] = a.epi.sw[col];
+            if (a.epi.bias != nullptr) my_bias[e] = a.epi.bias[col];
+          }
+        }
+      }
+      ok = mbar_wait(tfull_bar(acc), acc_phase, a.status, ERR_EPILOGUE);
+      if constexpr (F8) {
+        ok = epilogue_bar_and_n(n_epi_threads, ok);      // all go on or all leave; the tile before is done with its columns
+        if (!ok) break;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int c = epi_tid + e * n_epi_threads;
+          if (c < kPairBN) {
+            col_scale[c] = my_scale[e];
+            col_bias[c] = my_bias[e];
+          }
+        }
+        epilogue_bar_sync_n(n_epi_threads);
+      }
+      if (!ok) break;
       tc_fence_after();
       const int r_in_tile = quarter * 32 + lane;
       const int row = mt * 2 * BM + (int)rank * BM + r_in_tile;
@@ -1354,7 +1398,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairMaxThreads, 1)
                 for (int j = 0; j < 32; ++j) f[j] += __uint_as_float(v1[j]);
               }
             }
-            if (row_ok) epi_store_row32(a.epi, a.y, a.ldy, a.vec_store, row, col0, a.n, f, nullptr, &a.peers);
+            if (row_ok) epi_store_row32<F8>(a.epi, a.y, a.ldy, a.vec_store, row, col0, a.n, f, nullptr, &a.peers);
           }
         }
         tc_fence_before();
@@ -1362,7 +1406,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairMaxThreads, 1)
         if (lane == 0) mbar_arrive_cluster(tempty_bar(acc), 0);   // tensor memory no longer needed for this tile
         continue;
       }
-      if (epi_is_plain(a.epi)) {
+      if (!F8 && epi_is_plain(a.epi)) {
         __half* yrow = static_cast<__half*>(a.y) + (int64_t)row * a.ldy;
         // Four warps (the plain launch): 128 columns at a time go through shared memory, so that a warp
         // stores two whole rows of 256 contiguous bytes per instruction instead of 16 bytes of each of
@@ -1411,21 +1455,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairMaxThreads, 1)
       auto finish_chunk = [&](int c, const uint32_t* r, const ResChunk* res) {
         const int col0 = col_base + c * 32;
         const int blk0 = col_base + (c & ~1) * 32;
-        const bool staged_f = DTAS_PAIR_STAGED_STORE && a.vec_store && !a.epi.out_f32 && blk0 + 64 <= a.n && (c | 1) < c_end;
+        const bool whole = a.vec_store && blk0 + 64 <= a.n;
+        // e4m3: ragged edges and unaligned rows leave through the stage as well, element by element but row by row
+        const bool staged_f = DTAS_PAIR_STAGED_STORE && !a.epi.out_f32 && (whole || F8) && (c | 1) < c_end;
         float f[32];
 #pragma unroll
         for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(r[j]);
+        if constexpr (F8) epi_scale_bias_row32(a.epi, row_scale, col_scale + c * 32, col_bias + c * 32, f);
         if (staged_f) {
-          if (row_ok) epi_apply_row32(a.epi, row, col0, a.n, f, res);
+          if (row_ok && (!F8 || col0 < a.n)) epi_apply_row32<F8>(a.epi, row, col0, a.n, f, res, F8);
 #pragma unroll
           for (int q = 0; q < 4; ++q) stage_f[lane * 8 + (((c & 1) * 4 + q) ^ (lane & 7))] = epi_pack8(f + 8 * q);
           if (c & 1) {
             __syncwarp();
-            epi_store_staged_block<8>(stage_f, lane, mt * 2 * BM + (int)rank * BM + quarter * 32, a.m, a.y, a.ldy, blk0, a.peers);
+            if (!F8 || whole)
+              epi_store_staged_block<8>(stage_f, lane, mt * 2 * BM + (int)rank * BM + quarter * 32, a.m, a.y, a.ldy, blk0, a.peers);
+            else
+              epi_store_staged_elements<8>(stage_f, lane, mt * 2 * BM + (int)rank * BM + quarter * 32, a.m, a.y, a.ldy, blk0, a.n);
             __syncwarp();
           }
         } else if (row_ok && col0 < a.n) {
-          epi_store_row32(a.epi, a.y, a.ldy, a.vec_store, row, col0, a.n, f, res, &a.peers);
+          epi_store_row32<F8>(a.epi, a.y, a.ldy, a.vec_store, row, col0, a.n, f, res, &a.peers, F8);
         }
       };
       if (a.epi.res1 == nullptr) {
@@ -1525,7 +1575,7 @@ __device__ __forceinline__ void bulk_copy_to_peer(uint32_t dst_cluster, uint32_t
 }
 
 // a.m_tiles x a.n_tiles tiles of 128 x BN; grid = 2 x tiles; a.num_kb >= 2; a.splits is not used.
-template <int BN>
+template <int BN, bool F8>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     gemm_f16_tcgen05_k2_kernel(const __grid_constant__ CUtensorMap tmap_x,
                                const __grid_constant__ CUtensorMap tmap_w, const GemmArgs a) {
@@ -1602,7 +1652,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
         const uint32_t sa = base + stage * C::kStageBytes;
         const uint64_t da = make_kmajor_sw128_desc(sa);
         const uint64_t db = make_kmajor_sw128_desc(sa + C::kABytes);
-        umma_kblock(a.f8, tmem_base, da, db, idesc, kb == kb0);
+        umma_kblock<F8>(tmem_base, da, db, idesc, kb == kb0);
         umma_commit(empty_bar(stage));
         if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
       }
@@ -1656,7 +1706,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
               f[4 * q + 2] = __uint_as_float(r[4 * q + 2]) + v.z;
               f[4 * q + 3] = __uint_as_float(r[4 * q + 3]) + v.w;
             }
-            epi_store_row32(a.epi, a.y, a.ldy, a.vec_store, row, col0, a.n, f);
+            epi_store_row32<F8>(a.epi, a.y, a.ldy, a.vec_store, row, col0, a.n, f);
           }
         }
       }
@@ -1695,7 +1745,7 @@ struct SwapKcCfg {
 };
 
 // a.n_tiles 128-column tiles; grid = S x a.n_tiles; a.num_kb >= S.
-template <int MN, int S>
+template <int MN, int S, bool F8>
 __global__ void __cluster_dims__(S, 1, 1) __launch_bounds__(kGemmThreads, 1)
     gemm_f16_tcgen05_swap_kc_kernel(const __grid_constant__ CUtensorMap tmap_w,
                                     const __grid_constant__ CUtensorMap tmap_x, const GemmArgs a) {
@@ -1770,7 +1820,7 @@ __global__ void __cluster_dims__(S, 1, 1) __launch_bounds__(kGemmThreads, 1)
         const uint32_t sa = base + stage * C::kStageBytes;
         const uint64_t da = make_kmajor_sw128_desc(sa);
         const uint64_t db = make_kmajor_sw128_desc(sa + C::kWBytes);
-        umma_kblock(a.f8, tmem_base, da, db, idesc, kb == kb0);
+        umma_kblock<F8>(tmem_base, da, db, idesc, kb == kb0);
         umma_commit(empty_bar(stage));
         if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
       }
@@ -1832,7 +1882,7 @@ __global__ void __cluster_dims__(S, 1, 1) __launch_bounds__(kGemmThreads, 1)
                 f[4 * q] += v.x; f[4 * q + 1] += v.y; f[4 * q + 2] += v.z; f[4 * q + 3] += v.w;
               }
             }
-            epi_scale_bias_column<kChunk>(a.epi, c * kChunk, a.m, col, bias, f);
+            epi_scale_bias_column<F8, kChunk>(a.epi, c * kChunk, a.m, col, bias, f);
             epi_store_column<kChunk>(a.epi, a.y, a.ldy, c * kChunk, a.m, col, f);
           }
         }
@@ -1867,6 +1917,7 @@ __global__ void __launch_bounds__(256)
   const T* wr = w + (int64_t)col * k;
   float acc = 0.f;
   for (int i = 0; i < k; ++i) acc = fmaf(simt_f32(xr[i]), simt_f32(wr[i]), acc);
+  if constexpr (sizeof(T) == 1) acc = acc * epi.sx[row] * epi.sw[col];
   epi_store(epi, y, ldy, row, col, epi_value(epi, acc, row, col));
 }
 
@@ -2295,7 +2346,7 @@ GemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, int sm_count, bool tma_ok, c
   return p;
 }
 
-template <int BN>
+template <int BN, bool F8>
 int launch_tc(const CUtensorMap& tx, const CUtensorMap& tw, const GemmArgs& a, int sm_count,
               cudaStream_t st) {
   using C = Cfg<BN>;
@@ -2303,30 +2354,32 @@ int launch_tc(const CUtensorMap& tx, const CUtensorMap& tw, const GemmArgs& a, i
   int dev = 0;
   DTAS_CUDA(cudaGetDevice(&dev));
   if (dev < 64 && !attr_set[dev].load(std::memory_order_acquire)) {
-    DTAS_CUDA(cudaFuncSetAttribute(gemm_f16_tcgen05_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    DTAS_CUDA(cudaFuncSetAttribute((gemm_f16_tcgen05_kernel<BN, F8>), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    C::kSmemBytes));
     attr_set[dev].store(true, std::memory_order_release);
   }
   const int total = a.m_tiles * a.n_tiles * a.splits;
   int grid = total < sm_count ? total : sm_count;
   if (a.sk_per > 0) grid = (a.m_tiles * a.n_tiles * a.num_kb + a.sk_per - 1) / a.sk_per;
-  launch_kernel(gemm_f16_tcgen05_kernel<BN>, grid, kGemmThreads, C::kSmemBytes, st, tx, tw, a);
+  launch_kernel(gemm_f16_tcgen05_kernel<BN, F8>, grid, kGemmThreads, C::kSmemBytes, st, tx, tw, a);
   return after_launch("gemm_f16_tcgen05_kernel");
 }
 
+template <bool F8>
 int launch_pair(const CUtensorMap& tx, const CUtensorMap& tw, const GemmArgs& a, int sm_count, cudaStream_t st, bool stream_k) {
+  constexpr int kSmem = kPairSmemBytes + (F8 ? kPairColBytes : 0);
   static std::atomic<bool> attr_set[64];   // zero-initialised; set after the attribute call returned
   static int max_pairs[64] = {0};
   int dev = 0;
   DTAS_CUDA(cudaGetDevice(&dev));
   if (dev < 64 && !attr_set[dev].load(std::memory_order_acquire)) {
-    DTAS_CUDA(cudaFuncSetAttribute(gemm_f16_tcgen05_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   kPairSmemBytes));
+    DTAS_CUDA(cudaFuncSetAttribute(gemm_f16_tcgen05_pair_kernel<F8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   kSmem));
     // how many CTA pairs the device can hold at once (one CTA per SM, pairs share a TPC)
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * (unsigned)(sm_count / 2));
     cfg.blockDim = dim3(kPairMaxThreads);
-    cfg.dynamicSmemBytes = kPairSmemBytes;
+    cfg.dynamicSmemBytes = kSmem;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = 2;
@@ -2335,7 +2388,7 @@ int launch_pair(const CUtensorMap& tx, const CUtensorMap& tw, const GemmArgs& a,
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, gemm_f16_tcgen05_pair_kernel, &cfg) != cudaSuccess || n <= 0) {
+    if (cudaOccupancyMaxActiveClusters(&n, gemm_f16_tcgen05_pair_kernel<F8>, &cfg) != cudaSuccess || n <= 0) {
       (void)cudaGetLastError();
       n = sm_count / 2;
     }
@@ -2359,59 +2412,59 @@ int launch_pair(const CUtensorMap& tx, const CUtensorMap& tw, const GemmArgs& a,
   // twice the epilogue warps when there is an activation or a residual to work through per element, or
   // partial tiles to read back (the read rate of a CTA grows with the warps that issue the loads)
   const int threads = (epi_has_work(a.epi) || ap.sk_per > 0) ? kPairMaxThreads : kGemmThreads;
-  launch_kernel(gemm_f16_tcgen05_pair_kernel, 2 * pairs, threads, kPairSmemBytes, st, tx, tw, ap);
+  launch_kernel(gemm_f16_tcgen05_pair_kernel<F8>, 2 * pairs, threads, kSmem, st, tx, tw, ap);
   return after_launch("gemm_f16_tcgen05_pair_kernel");
 }
 
-template <int BN>
+template <int BN, bool F8>
 int launch_k2(const CUtensorMap& tx, const CUtensorMap& tw, const GemmArgs& a, cudaStream_t st) {
   using C = K2Cfg<BN>;
   static std::atomic<bool> attr_set[64];   // zero-initialised; set after the attribute call returned
   int dev = 0;
   DTAS_CUDA(cudaGetDevice(&dev));
   if (dev < 64 && !attr_set[dev].load(std::memory_order_acquire)) {
-    DTAS_CUDA(cudaFuncSetAttribute(gemm_f16_tcgen05_k2_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    DTAS_CUDA(cudaFuncSetAttribute((gemm_f16_tcgen05_k2_kernel<BN, F8>), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    C::kSmemBytes));
     attr_set[dev].store(true, std::memory_order_release);
   }
   const int64_t grid = 2ll * a.m_tiles * a.n_tiles;
   if (grid > 0x7fffffffLL) DTAS_FAIL(DTAS_EINVAL, "gemm: too many tiles");
-  launch_kernel(gemm_f16_tcgen05_k2_kernel<BN>, (unsigned)grid, kGemmThreads, C::kSmemBytes, st, tx, tw, a);
+  launch_kernel(gemm_f16_tcgen05_k2_kernel<BN, F8>, (unsigned)grid, kGemmThreads, C::kSmemBytes, st, tx, tw, a);
   return after_launch("gemm_f16_tcgen05_k2_kernel");
 }
 
-template <int MN, int S>
+template <int MN, int S, bool F8>
 int launch_swap_kc(const CUtensorMap& tw, const CUtensorMap& tx, const GemmArgs& a, cudaStream_t st) {
   using C = SwapKcCfg<MN>;
   static std::atomic<bool> attr_set[64];   // zero-initialised; set after the attribute call returned
   int dev = 0;
   DTAS_CUDA(cudaGetDevice(&dev));
   if (dev < 64 && !attr_set[dev].load(std::memory_order_acquire)) {
-    DTAS_CUDA(cudaFuncSetAttribute((gemm_f16_tcgen05_swap_kc_kernel<MN, S>), cudaFuncAttributeMaxDynamicSharedMemorySize,
+    DTAS_CUDA(cudaFuncSetAttribute((gemm_f16_tcgen05_swap_kc_kernel<MN, S, F8>), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    C::kSmemBytes));
     attr_set[dev].store(true, std::memory_order_release);
   }
   const int64_t grid = (int64_t)S * a.n_tiles;
   if (grid > 0x7fffffffLL) DTAS_FAIL(DTAS_EINVAL, "gemm: too many tiles");
-  launch_kernel(gemm_f16_tcgen05_swap_kc_kernel<MN, S>, (unsigned)grid, kGemmThreads, C::kSmemBytes, st, tw, tx, a);
+  launch_kernel(gemm_f16_tcgen05_swap_kc_kernel<MN, S, F8>, (unsigned)grid, kGemmThreads, C::kSmemBytes, st, tw, tx, a);
   return after_launch("gemm_f16_tcgen05_swap_kc_kernel");
 }
 
-template <int MN>
+template <int MN, bool F8>
 int launch_swap(const CUtensorMap& tw, const CUtensorMap& tx, const GemmArgs& a, int sm_count, cudaStream_t st) {
   using C = SwapCfg<MN>;
   static std::atomic<bool> attr_set[64];   // zero-initialised; set after the attribute call returned
   int dev = 0;
   DTAS_CUDA(cudaGetDevice(&dev));
   if (dev < 64 && !attr_set[dev].load(std::memory_order_acquire)) {
-    DTAS_CUDA(cudaFuncSetAttribute(gemm_f16_tcgen05_swap_kernel<MN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    DTAS_CUDA(cudaFuncSetAttribute((gemm_f16_tcgen05_swap_kernel<MN, F8>), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    C::kSmemBytes));
     attr_set[dev].store(true, std::memory_order_release);
   }
   const int total = a.n_tiles * a.splits;
   int grid = total < sm_count ? total : sm_count;
   if (a.sk_per > 0) grid = (a.n_tiles * a.num_kb + a.sk_per - 1) / a.sk_per;
-  launch_kernel(gemm_f16_tcgen05_swap_kernel<MN>, grid, kGemmThreads, C::kSmemBytes, st, tw, tx, a);
+  launch_kernel(gemm_f16_tcgen05_swap_kernel<MN, F8>, grid, kGemmThreads, C::kSmemBytes, st, tw, tx, a);
   return after_launch("gemm_f16_tcgen05_swap_kernel");
 }
 
@@ -2580,6 +2633,49 @@ static int finish_epilogue(Epilogue& e, const void* y, int64_t ldy) {
   return (aligned16(y) && ldy % (e.out_f32 ? 4 : 8) == 0) ? 1 : 0;
 }
 
+// The kernel of a plan, for operands of either width.
+template <bool F8>
+static int launch_planned(const GemmPlan& p, const CUtensorMap& tx, const CUtensorMap& tw, GemmArgs a, int sm_count, cudaStream_t st) {
+  if (p.k2) return p.bn == 128 ? launch_k2<128, F8>(tx, tw, a, st) : launch_k2<64, F8>(tx, tw, a, st);
+  if (p.pair) {
+    a.m_tiles = (a.m + 2 * BM - 1) / (2 * BM);
+    a.n_tiles = (a.n + kPairBN - 1) / kPairBN;
+    return launch_pair<F8>(tx, tw, a, sm_count, st, p.pair_sk);
+  }
+  if (p.swap_mn > 0) {
+    a.m_tiles = 1;
+    a.n_tiles = (a.n + BM - 1) / BM;
+    a.sk_per = p.sk_per;
+    a.slots_cap = p.slots_cap;
+    if (p.kc > 0) {
+      const int code = (p.swap_mn == 16 ? 0 : (p.swap_mn == 32 ? 10 : 20)) + p.kc;
+      switch (code) {
+        case 2: return launch_swap_kc<16, 2, F8>(tw, tx, a, st);
+        case 3: return launch_swap_kc<16, 3, F8>(tw, tx, a, st);
+        case 4: return launch_swap_kc<16, 4, F8>(tw, tx, a, st);
+        case 12: return launch_swap_kc<32, 2, F8>(tw, tx, a, st);
+        case 13: return launch_swap_kc<32, 3, F8>(tw, tx, a, st);
+        case 14: return launch_swap_kc<32, 4, F8>(tw, tx, a, st);
+        case 22: return launch_swap_kc<64, 2, F8>(tw, tx, a, st);
+        case 23: return launch_swap_kc<64, 3, F8>(tw, tx, a, st);
+        default: return launch_swap_kc<64, 4, F8>(tw, tx, a, st);
+      }
+    }
+    switch (p.swap_mn) {
+      case 16: return launch_swap<16, F8>(tw, tx, a, sm_count, st);
+      case 32: return launch_swap<32, F8>(tw, tx, a, sm_count, st);
+      case 64: return launch_swap<64, F8>(tw, tx, a, sm_count, st);
+      case 128: return launch_swap<128, F8>(tw, tx, a, sm_count, st);
+      default: return launch_swap<256, F8>(tw, tx, a, sm_count, st);
+    }
+  }
+  switch (p.bn) {
+    case 256: return launch_tc<256, F8>(tx, tw, a, sm_count, st);
+    case 128: return launch_tc<128, F8>(tx, tw, a, sm_count, st);
+    default: return launch_tc<64, F8>(tx, tw, a, sm_count, st);
+  }
+}
+
 int launch_gemm(const void* x, const void* w, const Epilogue& epi, void* y, int64_t m, int64_t n,
                 int64_t k, int64_t ldy, DeviceCtx* ctx, cudaStream_t st, const PeerOut* peers, bool f8) {
   if (m > 0x7fffffffLL / 2 || n > 0x7fffffffLL / 2 || k > 0x7fffffffLL / 2)
@@ -2642,7 +2738,6 @@ int launch_gemm(const void* x, const void* w, const Epilogue& epi, void* y, int6
   a.kb_per_split = p.kb_per_split;
   a.num_kb = (int)((k + BK - 1) / BK);
   a.vec_store = finish_epilogue(a.epi, y, ldy);
-  a.f8 = f8 ? 1 : 0;
   if (scatter) {
     a.peers = *peers;
     for (int j = 0; j < peers->n; ++j)
@@ -2650,44 +2745,7 @@ int launch_gemm(const void* x, const void* w, const Epilogue& epi, void* y, int6
   }
   if ((int64_t)a.m_tiles * a.n_tiles * a.splits > 0x7fffffffLL)
     DTAS_FAIL(DTAS_EINVAL, "gemm: too many tiles");
-  if (p.k2) return p.bn == 128 ? launch_k2<128>(tx, tw, a, st) : launch_k2<64>(tx, tw, a, st);
-  if (p.pair) {
-    a.m_tiles = (int)((m + 2 * BM - 1) / (2 * BM));
-    a.n_tiles = (int)((n + kPairBN - 1) / kPairBN);
-    return launch_pair(tx, tw, a, ctx->sm_count, st, p.pair_sk);
-  }
-  if (p.swap_mn > 0) {
-    a.m_tiles = 1;
-    a.n_tiles = (int)((n + BM - 1) / BM);
-    a.sk_per = p.sk_per;
-    a.slots_cap = p.slots_cap;
-    if (p.kc > 0) {
-      const int code = (p.swap_mn == 16 ? 0 : (p.swap_mn == 32 ? 10 : 20)) + p.kc;
-      switch (code) {
-        case 2: return launch_swap_kc<16, 2>(tw, tx, a, st);
-        case 3: return launch_swap_kc<16, 3>(tw, tx, a, st);
-        case 4: return launch_swap_kc<16, 4>(tw, tx, a, st);
-        case 12: return launch_swap_kc<32, 2>(tw, tx, a, st);
-        case 13: return launch_swap_kc<32, 3>(tw, tx, a, st);
-        case 14: return launch_swap_kc<32, 4>(tw, tx, a, st);
-        case 22: return launch_swap_kc<64, 2>(tw, tx, a, st);
-        case 23: return launch_swap_kc<64, 3>(tw, tx, a, st);
-        default: return launch_swap_kc<64, 4>(tw, tx, a, st);
-      }
-    }
-    switch (p.swap_mn) {
-      case 16: return launch_swap<16>(tw, tx, a, ctx->sm_count, st);
-      case 32: return launch_swap<32>(tw, tx, a, ctx->sm_count, st);
-      case 64: return launch_swap<64>(tw, tx, a, ctx->sm_count, st);
-      case 128: return launch_swap<128>(tw, tx, a, ctx->sm_count, st);
-      default: return launch_swap<256>(tw, tx, a, ctx->sm_count, st);
-    }
-  }
-  switch (p.bn) {
-    case 256: return launch_tc<256>(tx, tw, a, ctx->sm_count, st);
-    case 128: return launch_tc<128>(tx, tw, a, ctx->sm_count, st);
-    default: return launch_tc<64>(tx, tw, a, ctx->sm_count, st);
-  }
+  return f8 ? launch_planned<true>(p, tx, tw, a, ctx->sm_count, st) : launch_planned<false>(p, tx, tw, a, ctx->sm_count, st);
 }
 
 void gemm_f8_variant_name(int64_t m, int64_t n, int64_t k, const DeviceCtx* ctx, char* buf, int len) {
@@ -2920,9 +2978,9 @@ extern "C" int dtas_gemm_nt_static_scratch(const void* x, const void* w, const v
   a.num_kb = (int)((k + BK - 1) / BK);
   a.vec_store = finish_epilogue(a.epi, y, ldy);
   switch (sp.bn) {
-    case 256: return launch_tc<256>(tx, tw, a, sd->sm_count, st);
-    case 128: return launch_tc<128>(tx, tw, a, sd->sm_count, st);
-    default: return launch_tc<64>(tx, tw, a, sd->sm_count, st);
+    case 256: return launch_tc<256, false>(tx, tw, a, sd->sm_count, st);
+    case 128: return launch_tc<128, false>(tx, tw, a, sd->sm_count, st);
+    default: return launch_tc<64, false>(tx, tw, a, sd->sm_count, st);
   }
 }
 
