@@ -310,8 +310,8 @@ __device__ __forceinline__ void epi_scale_bias_row32(const Epilogue& e, float sx
 
 // The arithmetic of the tail on 32 consecutive columns of one row, in place: scales of 8-bit operands, bias,
 // activation, residuals.  `pre`, when given, holds the residual values of this chunk fetched earlier; `scaled`:
-// scales and bias have been applied (epi_scale_bias_row32).
-template <bool F8>
+// scales and bias have been applied (epi_scale_bias_row32); RES false: there are no residuals.
+template <bool F8, bool RES = true>
 __device__ __forceinline__ void epi_apply_row32(const Epilogue& e, int64_t row, int col0, int n, float* acc32,
                                                 const ResChunk* pre = nullptr, bool scaled = false) {
   if (!scaled) {
@@ -322,6 +322,7 @@ __device__ __forceinline__ void epi_apply_row32(const Epilogue& e, int64_t row, 
 #pragma unroll
     for (int g = 0; g < 32; g += 8) gelu_erf_n<8>(acc32 + g);   // groups of 4 time the same, of 16 slower
   }
+  if constexpr (!RES) return;
   if (pre != nullptr) {
     epi_add_vec32(pre->v[0], acc32);
     if (e.res2 != nullptr) epi_add_vec32(pre->v[1], acc32);
@@ -396,12 +397,12 @@ __device__ __forceinline__ void epi_store_staged_elements(const uint4* stage, in
 // Finishes 32 consecutive output columns col0 .. col0+31 of one row held in acc32 (fp32 dot
 // products) and stores them.  vec_store: 16-byte stores into Y rows are aligned.  `pre`, when
 // given, holds the residual values of this chunk fetched earlier (epi_prefetch_res32).
-template <bool F8>
+template <bool F8, bool RES = true>
 __device__ __forceinline__ void epi_store_row32(const Epilogue& e, void* y, int64_t ldy, int vec_store, int64_t row,
                                                 int col0, int n, float* acc32, const ResChunk* pre = nullptr,
                                                 const PeerOut* peers = nullptr, bool scaled = false) {
   const int n_peers = peers != nullptr ? peers->n : 0;
-  epi_apply_row32<F8>(e, row, col0, n, acc32, pre, scaled);
+  epi_apply_row32<F8, RES>(e, row, col0, n, acc32, pre, scaled);
   const bool full = vec_store && col0 + 32 <= n;
   if (!e.out_f32) {
     __half* yrow = static_cast<__half*>(y) + row * ldy;

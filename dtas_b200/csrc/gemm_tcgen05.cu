@@ -1147,7 +1147,9 @@ constexpr int kPairMaxThreads = 32 * (2 + 8);   // producer, MMA issuer and up t
 // activation or residuals to work through: of the two warps that share a quarter of the tensor-memory
 // lanes one then finishes columns 0..127 of the tile and the other columns 128..255, so the tail of a
 // 256 x 256 tile is spread over twice the issue slots and hides behind a shorter main loop.
-template <bool F8>
+// RES: an e4m3 instantiation with or without residuals, since the registers of the one cost the other 2 to 9 % (a test
+// of the arguments decides for fp16 operands).
+template <bool F8, bool RES>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairMaxThreads, 1)
     gemm_f16_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_x,
                                  const __grid_constant__ CUtensorMap tmap_w, const GemmArgs a) {
@@ -1463,7 +1465,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairMaxThreads, 1)
         for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(r[j]);
         if constexpr (F8) epi_scale_bias_row32(a.epi, row_scale, col_scale + c * 32, col_bias + c * 32, f);
         if (staged_f) {
-          if (row_ok && (!F8 || col0 < a.n)) epi_apply_row32<F8>(a.epi, row, col0, a.n, f, res, F8);
+          if (row_ok && (!F8 || col0 < a.n)) epi_apply_row32<F8, !F8 || RES>(a.epi, row, col0, a.n, f, res, F8);
 #pragma unroll
           for (int q = 0; q < 4; ++q) stage_f[lane * 8 + (((c & 1) * 4 + q) ^ (lane & 7))] = epi_pack8(f + 8 * q);
           if (c & 1) {
@@ -1475,10 +1477,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairMaxThreads, 1)
             __syncwarp();
           }
         } else if (row_ok && col0 < a.n) {
-          epi_store_row32<F8>(a.epi, a.y, a.ldy, a.vec_store, row, col0, a.n, f, res, &a.peers, F8);
+          epi_store_row32<F8, !F8 || RES>(a.epi, a.y, a.ldy, a.vec_store, row, col0, a.n, f, res, &a.peers, F8);
         }
       };
-      if (a.epi.res1 == nullptr) {
+      if (F8 ? !RES : a.epi.res1 == nullptr) {
         // Activation without residuals: the accumulator words of the next chunk are on their way from
         // tensor memory while the current chunk is worked on (two sets of registers in turn).
         uint32_t ra[32], rb[32];
@@ -1498,6 +1500,48 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairMaxThreads, 1)
             tmem_ld_wait();
             tmem_ld_landed(ra);
           }
+        }
+      } else if (F8) {
+        // Residuals beside e4m3 operands: blocks of 64 columns of the first come in by rows (a load instruction covers
+        // four 128-byte lines, not 32 pieces of 16 bytes), a block ahead, and are laid out in the stage, where the
+        // results then take their places.  Ragged and unaligned ones are read in place.
+        const bool by_rows = DTAS_PAIR_STAGED_STORE && a.epi.vec_res && a.vec_store && !a.epi.out_f32 &&
+                             col_base + c_end * 32 <= a.n && (c_end & 1) == 0;
+        const int row0 = mt * 2 * BM + (int)rank * BM + quarter * 32;
+        uint4 ahead[8];
+        auto fetch = [&](int c) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int64_t rr = row0 + 4 * i + (lane >> 3);
+            if (rr < a.m) ahead[i] = *reinterpret_cast<const uint4*>(a.epi.res1 + rr * a.epi.ldr + col_base + c * 32 + 8 * (lane & 7));
+          }
+        };
+        if (by_rows) fetch(c_begin);
+#pragma unroll 1
+        for (int c = c_begin; c < c_end; ++c) {
+          if (by_rows && (c & 1) == 0) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int rl = 4 * i + (lane >> 3);
+              stage_f[rl * 8 + ((lane & 7) ^ (rl & 7))] = ahead[i];
+            }
+            if (c + 2 < c_end) fetch(c + 2);
+            __syncwarp();
+          }
+          uint32_t r[32];
+          tmem_ld32(t_addr + c * 32, r);
+          ResChunk r_now;
+          if (by_rows) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) r_now.v[0][q] = stage_f[lane * 8 + (((c & 1) * 4 + q) ^ (lane & 7))];
+            if (a.epi.res2 != nullptr && row_ok) {
+              const uint4* s2 = reinterpret_cast<const uint4*>(a.epi.res2 + (int64_t)row * a.epi.ldr + col_base + c * 32);
+#pragma unroll
+              for (int q = 0; q < 4; ++q) r_now.v[1][q] = s2[q];
+            }
+          }
+          tmem_ld_wait();
+          finish_chunk(c, r, by_rows ? &r_now : nullptr);
         }
       } else {
         // Residual rows are fetched two chunks ahead of their use.
@@ -2365,7 +2409,7 @@ int launch_tc(const CUtensorMap& tx, const CUtensorMap& tw, const GemmArgs& a, i
   return after_launch("gemm_f16_tcgen05_kernel");
 }
 
-template <bool F8>
+template <bool F8, bool RES>
 int launch_pair(const CUtensorMap& tx, const CUtensorMap& tw, const GemmArgs& a, int sm_count, cudaStream_t st, bool stream_k) {
   constexpr int kSmem = kPairSmemBytes + (F8 ? kPairColBytes : 0);
   static std::atomic<bool> attr_set[64];   // zero-initialised; set after the attribute call returned
@@ -2373,7 +2417,7 @@ int launch_pair(const CUtensorMap& tx, const CUtensorMap& tw, const GemmArgs& a,
   int dev = 0;
   DTAS_CUDA(cudaGetDevice(&dev));
   if (dev < 64 && !attr_set[dev].load(std::memory_order_acquire)) {
-    DTAS_CUDA(cudaFuncSetAttribute(gemm_f16_tcgen05_pair_kernel<F8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    DTAS_CUDA(cudaFuncSetAttribute((gemm_f16_tcgen05_pair_kernel<F8, RES>), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    kSmem));
     // how many CTA pairs the device can hold at once (one CTA per SM, pairs share a TPC)
     cudaLaunchConfig_t cfg = {};
@@ -2388,7 +2432,7 @@ int launch_pair(const CUtensorMap& tx, const CUtensorMap& tw, const GemmArgs& a,
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, gemm_f16_tcgen05_pair_kernel<F8>, &cfg) != cudaSuccess || n <= 0) {
+    if (cudaOccupancyMaxActiveClusters(&n, gemm_f16_tcgen05_pair_kernel<F8, RES>, &cfg) != cudaSuccess || n <= 0) {
       (void)cudaGetLastError();
       n = sm_count / 2;
     }
@@ -2412,7 +2456,7 @@ int launch_pair(const CUtensorMap& tx, const CUtensorMap& tw, const GemmArgs& a,
   // twice the epilogue warps when there is an activation or a residual to work through per element, or
   // partial tiles to read back (the read rate of a CTA grows with the warps that issue the loads)
   const int threads = (epi_has_work(a.epi) || ap.sk_per > 0) ? kPairMaxThreads : kGemmThreads;
-  launch_kernel(gemm_f16_tcgen05_pair_kernel<F8>, 2 * pairs, threads, kSmem, st, tx, tw, ap);
+  launch_kernel(gemm_f16_tcgen05_pair_kernel<F8, RES>, 2 * pairs, threads, kSmem, st, tx, tw, ap);
   return after_launch("gemm_f16_tcgen05_pair_kernel");
 }
 
@@ -2640,7 +2684,8 @@ static int launch_planned(const GemmPlan& p, const CUtensorMap& tx, const CUtens
   if (p.pair) {
     a.m_tiles = (a.m + 2 * BM - 1) / (2 * BM);
     a.n_tiles = (a.n + kPairBN - 1) / kPairBN;
-    return launch_pair<F8>(tx, tw, a, sm_count, st, p.pair_sk);
+    if (F8 && a.epi.res1 != nullptr) return launch_pair<F8, F8>(tx, tw, a, sm_count, st, p.pair_sk);
+    return launch_pair<F8, false>(tx, tw, a, sm_count, st, p.pair_sk);
   }
   if (p.swap_mn > 0) {
     a.m_tiles = 1;
