@@ -310,7 +310,7 @@ int dtas_add_rms_norm(const void* x, const void* res, const void* weight, void* 
   if (out_dtype != DTAS_F16) DTAS_NONNULL("add_rms_norm", scale);
   Call c;
   if ((rc = c.begin(device, stream))) return rc;
-  return launch_add_rms_norm(x, res, weight, y, res_out, scale, m, n_cols, eps, in_dtype, out_dtype, c.stream);
+  return launch_add_rms_norm(x, res, weight, y, res_out, scale, m, n_cols, eps, in_dtype, out_dtype, c.ctx, c.stream);
 }
 
 int dtas_quantize(const void* x, void* q, float* scale, int64_t m, int64_t n_cols, int in_dtype, int out_dtype,
@@ -326,7 +326,7 @@ int dtas_quantize(const void* x, void* q, float* scale, int64_t m, int64_t n_col
     DTAS_FAIL(DTAS_EUNSUPPORTED, "quantize: the output is int8 or e4m3 (dtype %d)", out_dtype);
   Call c;
   if ((rc = c.begin(device, stream))) return rc;
-  return launch_quantize(x, q, scale, m, n_cols, in_dtype, out_dtype, c.stream);
+  return launch_quantize(x, q, scale, m, n_cols, in_dtype, out_dtype, c.ctx, c.stream);
 }
 
 int dtas_gemv_w4(const void* x, const float* x_scale, const void* w, const void* w_scale, const void* w_zero,

@@ -23,6 +23,8 @@
 // element throughout).
 #include <cuda_fp8.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace dtas {
@@ -237,53 +239,15 @@ __device__ __forceinline__ float quant_scale(float top, float r, float q) {
   return top < INFINITY ? (top * r) / q : __int_as_float(0x7fc00000);
 }
 
+// A row whose elements - for the norm, their sums with the residual - are in registers: its results.
 template <int OP, typename InT, typename OutT, int VEC, int CH, bool EDGE>
-__global__ void __launch_bounds__(max_threads(VEC, CH)) row_quant_kernel(const RowArgs a) {
-  __shared__ float2 ex[kMaxThreads / 32];
+__device__ __forceinline__ void finish_row(const RowArgs& a, int64_t row, bool live, int n, const int* at, float (*v)[VEC],
+                                           const Weights<VEC, EDGE>* wt, float2* ex) {
   constexpr bool kNorm = OP == Q_NORM;
   constexpr bool k8 = sizeof(OutT) == 1;
-  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  const bool live = row < a.m;
-  const int n = live ? (int)a.n_cols : 0;
-  const int64_t off = (live ? row : 0) * a.n_cols;
-  const int lead = EDGE ? (int)(off & (VEC - 1)) : 0;      // elements of its first chunk that are not the row's
-  const InT* x = static_cast<const InT*>(a.x) + off;
-  int at[CH];
-#pragma unroll
-  for (int c = 0; c < CH; ++c) at[c] = (c * blockDim.x + threadIdx.x) * VEC - lead;
-
-  pdl_wait();
-  pdl_launch_dependents();
-  float v[CH][VEC];
-#pragma unroll
-  for (int c = 0; c < CH; ++c) {
-    if (at[c] < n) {
-      load_chunk<VEC, EDGE>(x, at[c], n, v[c]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) v[c][i] = 0.f;
-    }
-  }
-  Weights<VEC, EDGE> wt[CH];
-  if constexpr (kNorm) {
-#pragma unroll
-    for (int c = 0; c < CH; ++c)
-      if (at[c] < n) wt[c].load(a.weight, at[c], n);
-  }
+  const int64_t off = row * a.n_cols;
   float sum = 0.f, top = 0.f;
   if constexpr (kNorm) {
-    if (a.res != nullptr) {
-      const InT* res = static_cast<const InT*>(a.res) + off;
-#pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        if (at[c] < n) {
-          float t[VEC];
-          load_chunk<VEC, EDGE>(res, at[c], n, t);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) v[c][i] += t[i];
-        }
-      }
-    }
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
 #pragma unroll
@@ -330,6 +294,130 @@ __global__ void __launch_bounds__(max_threads(VEC, CH)) row_quant_kernel(const R
         store_chunk<VEC, EDGE>(reinterpret_cast<__half*>(y), at[c], n, o);
       }
     }
+  }
+}
+
+template <int OP, typename InT, typename OutT, int VEC, int CH, bool EDGE>
+__global__ void __launch_bounds__(max_threads(VEC, CH)) row_quant_kernel(const RowArgs a) {
+  __shared__ float2 ex[kMaxThreads / 32];
+  constexpr bool kNorm = OP == Q_NORM;
+  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  const bool live = row < a.m;
+  const int n = live ? (int)a.n_cols : 0;
+  const int64_t off = (live ? row : 0) * a.n_cols;
+  const int lead = EDGE ? (int)(off & (VEC - 1)) : 0;      // elements of its first chunk that are not the row's
+  const InT* x = static_cast<const InT*>(a.x) + off;
+  int at[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) at[c] = (c * blockDim.x + threadIdx.x) * VEC - lead;
+
+  pdl_wait();
+  pdl_launch_dependents();
+  float v[CH][VEC];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    if (at[c] < n) {
+      load_chunk<VEC, EDGE>(x, at[c], n, v[c]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[c][i] = 0.f;
+    }
+  }
+  Weights<VEC, EDGE> wt[CH];
+  if constexpr (kNorm) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+      if (at[c] < n) wt[c].load(a.weight, at[c], n);
+  }
+  if constexpr (kNorm) {
+    if (a.res != nullptr) {
+      const InT* res = static_cast<const InT*>(a.res) + off;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        if (at[c] < n) {
+          float t[VEC];
+          load_chunk<VEC, EDGE>(res, at[c], n, t);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) v[c][i] += t[i];
+        }
+      }
+    }
+  }
+  finish_row<OP, InT, OutT, VEC, CH, EDGE>(a, row, live, n, at, v, wt, ex);
+}
+
+// Sixteen-byte vectors of eight consecutive elements as loaded.
+template <typename T>
+struct Raw8 {
+  uint4 r[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void get(float* v) const {
+    const T* e = reinterpret_cast<const T*>(r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
+  }
+};
+
+// Many rows: the CTAs that fit on the device take rows in turn, and a row's loads are under way while the one before
+// it is reduced and stored; the weights stay in registers.
+template <int OP, typename InT, typename OutT, int CH>
+__global__ void __launch_bounds__(512) row_quant_stream_kernel(const RowArgs a) {
+  __shared__ float2 ex[2][kMaxThreads / 32];       // in turn: a row's exchange cannot meet the one before it
+  constexpr bool kNorm = OP == Q_NORM;
+  const int n = (int)a.n_cols;
+  int at[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) at[c] = (c * blockDim.x + threadIdx.x) * 8;
+  const int64_t step = (int64_t)gridDim.x * blockDim.y;
+  int64_t first = (int64_t)blockIdx.x * blockDim.y;
+
+  pdl_wait();
+  pdl_launch_dependents();
+  Raw8<InT> x[CH], res[CH];
+  auto fetch = [&](int64_t row) {
+    if (row >= a.m) return;
+    const InT* px = static_cast<const InT*>(a.x) + row * a.n_cols;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+      if (at[c] < n) x[c].load(px + at[c]);
+    if (kNorm && a.res != nullptr) {
+      const InT* pr = static_cast<const InT*>(a.res) + row * a.n_cols;
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+        if (at[c] < n) res[c].load(pr + at[c]);
+    }
+  };
+  fetch(first + threadIdx.y);
+  Weights<8, false> wt[CH];
+  if constexpr (kNorm) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+      if (at[c] < n) wt[c].load(a.weight, at[c], n);
+  }
+  for (int turn = 0; first < a.m; first += step, turn ^= 1) {
+    const int64_t row = first + threadIdx.y;
+    const bool live = row < a.m;
+    float v[CH][8];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      if (live && at[c] < n) {
+        x[c].get(v[c]);
+        if (kNorm && a.res != nullptr) {
+          float t[8];
+          res[c].get(t);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[c][i] += t[i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[c][i] = 0.f;
+      }
+    }
+    fetch(row + step);
+    finish_row<OP, InT, OutT, 8, CH, false>(a, row, live, live ? n : 0, at, v, wt, ex[turn]);
   }
 }
 
@@ -387,10 +475,11 @@ struct RowPlan {
   int tpr;       // threads per row
   int rows;      // rows per CTA
   bool edge;     // rows that start inside a vector
+  bool stream;   // row_quant_stream_kernel
 };
 
-inline RowPlan row_plan(int64_t m, int64_t n_cols, bool aligned, bool norm) {
-  RowPlan p{0, 0, 0, 0, false};
+inline RowPlan row_plan(int64_t m, int64_t n_cols, bool aligned, bool norm, bool wide) {   // wide: fp32 inputs
+  RowPlan p{0, 0, 0, 0, false, false};
   p.vec = aligned ? 8 : 1;
   p.edge = aligned && n_cols % 8 != 0;
   const int64_t chunks = (n_cols + p.vec - 1) / p.vec + (p.edge ? 1 : 0);
@@ -408,19 +497,55 @@ inline RowPlan row_plan(int64_t m, int64_t n_cols, bool aligned, bool norm) {
     p.ch = m <= 592 || norm ? 1 : (chunks <= 128 ? 2 : 4);
     while (chunks > (int64_t)p.ch * max_threads(8, p.ch)) p.ch *= 2;
   }
+  // Rows in turn, four chunks to a thread (as many as leave it whole warps): fp16 norms of enough elements to fill the
+  // device a few times over - [8192, 4096] to e4m3 49 us a row per CTA, 40 us in turn; [900, 4096] 8.0 and 7.5; [600, 16384]
+  // 23.6 and 15.2; but [900, 1024] 3.3 and 3.6, and fp32 norms, whose rows in flight take twice the registers, 33 and 42
+  // at [4096, 4096].  For quantize only short rows gain, by the launches of so many CTAs: [8192, 1024] 9.0 and 6.6 us,
+  // [1500, 1024] 2.6 and 2.7, [8192, 4096] 17.8 and 18.0.
+  if (aligned && !p.edge) {
+    if (norm && !wide && m * n_cols > 2400000 && chunks <= 4 * 512) {
+      p.stream = true;
+      p.ch = chunks >= 128 ? 4 : (chunks >= 64 ? 2 : 1);
+    } else if (!norm && m > 4096 && chunks <= 128) {
+      p.stream = true;
+      p.ch = 2;
+    }
+  }
   p.tpr = (int)((chunks + p.ch - 1) / p.ch + 31) / 32 * 32;
   p.rows = p.tpr >= 64 ? 1 : 64 / p.tpr;
   return p;
 }
 
+template <int OP, typename InT, typename OutT, int CH>
+int launch_stream(const RowPlan& p, const RowArgs& a, int sm_count, cudaStream_t st) {
+  static std::atomic<int> per_sm[kMaxThreads / 32 + 1];      // CTAs of so many warps that an SM holds, once asked for
+  const int threads = p.tpr * p.rows;
+  int fit = per_sm[threads / 32].load(std::memory_order_relaxed);
+  if (fit == 0) {
+    DTAS_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, row_quant_stream_kernel<OP, InT, OutT, CH>, threads, 0));
+    per_sm[threads / 32].store(fit, std::memory_order_relaxed);
+  }
+  const int64_t groups = (a.m + p.rows - 1) / p.rows, most = (int64_t)sm_count * fit;
+  launch_kernel(row_quant_stream_kernel<OP, InT, OutT, CH>, (unsigned)(groups < most ? groups : most), dim3(p.tpr, p.rows), 0,
+                st, a);
+  return after_launch("row_quant_stream_kernel");
+}
+
 template <int OP, typename InT, typename OutT>
-int launch_typed(const RowPlan& p, const RowArgs& a, cudaStream_t st) {
+int launch_typed(const RowPlan& p, const RowArgs& a, int sm_count, cudaStream_t st) {
   const dim3 block(p.tpr, p.rows);
   const int64_t grid = (a.m + p.rows - 1) / p.rows;
   if (grid > 0x7fffffffLL) DTAS_FAIL(DTAS_EINVAL, "row op: too many rows (%lld)", (long long)a.m);
   if (p.vec == 0) {
     launch_kernel(row_quant_long_kernel<OP, InT, OutT>, (unsigned)grid, block, 0, st, a);
     return after_launch("row_quant_long_kernel");
+  }
+  if (p.stream) {
+    if constexpr (OP == Q_NORM && sizeof(InT) == 2) {
+      if (p.ch == 1) return launch_stream<OP, InT, OutT, 1>(p, a, sm_count, st);
+      if (p.ch == 4) return launch_stream<OP, InT, OutT, 4>(p, a, sm_count, st);
+    }
+    if constexpr (OP == Q_QUANT || sizeof(InT) == 2) return launch_stream<OP, InT, OutT, 2>(p, a, sm_count, st);
   }
 #define DTAS_ROWQ_CASE(V, C, E)                                                                    \
   if (p.vec == V && p.ch == C && p.edge == E) {                                                    \
@@ -435,43 +560,46 @@ int launch_typed(const RowPlan& p, const RowArgs& a, cudaStream_t st) {
 }
 
 template <int OP, typename InT>
-int launch_out(const RowPlan& p, const RowArgs& a, int out_dtype, cudaStream_t st) {
-  if (out_dtype == DTAS_E4M3) return launch_typed<OP, InT, __nv_fp8_e4m3>(p, a, st);
-  if (out_dtype == DTAS_I8) return launch_typed<OP, InT, int8_t>(p, a, st);
+int launch_out(const RowPlan& p, const RowArgs& a, int out_dtype, int sm_count, cudaStream_t st) {
+  if (out_dtype == DTAS_E4M3) return launch_typed<OP, InT, __nv_fp8_e4m3>(p, a, sm_count, st);
+  if (out_dtype == DTAS_I8) return launch_typed<OP, InT, int8_t>(p, a, sm_count, st);
   if constexpr (OP == Q_NORM) {
-    if (out_dtype == DTAS_F16) return launch_typed<OP, InT, __half>(p, a, st);
+    if (out_dtype == DTAS_F16) return launch_typed<OP, InT, __half>(p, a, sm_count, st);
   }
   DTAS_FAIL(DTAS_EUNSUPPORTED, "row op: unsupported output dtype %d", out_dtype);
 }
 
 template <int OP>
-int launch_in(const RowArgs& a, int in_dtype, int out_dtype, cudaStream_t st) {
+int launch_in(const RowArgs& a, int in_dtype, int out_dtype, int sm_count, cudaStream_t st) {
   // with rows that start inside a vector the weights are read one by one
   bool aligned = aligned16(a.x) && aligned16(a.res) && aligned16(a.res_out) && (a.n_cols % 8 != 0 || aligned16(a.weight));
   aligned = aligned && (reinterpret_cast<uintptr_t>(a.y) & (out_dtype == DTAS_F16 ? 15 : 7)) == 0;
-  const RowPlan p = row_plan(a.m, a.n_cols, aligned, OP == Q_NORM);
-  if (in_dtype == DTAS_F16) return launch_out<OP, __half>(p, a, out_dtype, st);
-  if (in_dtype == DTAS_F32) return launch_out<OP, float>(p, a, out_dtype, st);
+  const RowPlan p = row_plan(a.m, a.n_cols, aligned, OP == Q_NORM, in_dtype == DTAS_F32);
+  if (in_dtype == DTAS_F16) return launch_out<OP, __half>(p, a, out_dtype, sm_count, st);
+  if (in_dtype == DTAS_F32) return launch_out<OP, float>(p, a, out_dtype, sm_count, st);
   DTAS_FAIL(DTAS_EUNSUPPORTED, "row op: unsupported input dtype %d", in_dtype);
 }
 
 }  // namespace
 
 int launch_add_rms_norm(const void* x, const void* res, const void* weight, void* y, void* res_out, float* scale,
-                        int64_t m, int64_t n_cols, float eps, int in_dtype, int out_dtype, cudaStream_t st) {
+                        int64_t m, int64_t n_cols, float eps, int in_dtype, int out_dtype, const DeviceCtx* ctx, cudaStream_t st) {
   return launch_in<Q_NORM>(RowArgs{x, res, static_cast<const __half*>(weight), y, res_out, scale, m, n_cols, eps},
-                           in_dtype, out_dtype, st);
+                           in_dtype, out_dtype, ctx->sm_count, st);
 }
 
 int launch_quantize(const void* x, void* q, float* scale, int64_t m, int64_t n_cols, int in_dtype, int out_dtype,
-                    cudaStream_t st) {
-  return launch_in<Q_QUANT>(RowArgs{x, nullptr, nullptr, q, nullptr, scale, m, n_cols, 0.f}, in_dtype, out_dtype, st);
+                    const DeviceCtx* ctx, cudaStream_t st) {
+  return launch_in<Q_QUANT>(RowArgs{x, nullptr, nullptr, q, nullptr, scale, m, n_cols, 0.f}, in_dtype, out_dtype,
+                            ctx->sm_count, st);
 }
 
 void row_quant_variant_name(const char* op, int64_t m, int64_t n_cols, char* buf, int len) {
-  const RowPlan p = row_plan(m, n_cols, true, strcmp(op, "quantize") != 0);
-  if (p.vec == 0) snprintf(buf, len, "%s_long_cta%d", op, p.tpr);
-  else snprintf(buf, len, "%s_vec%d%s_tpr%d_ch%d", op, p.vec, p.edge ? "_edge" : "", p.tpr, p.ch);
+  const RowPlan p = row_plan(m, n_cols, true, strcmp(op, "quantize") != 0, false);
+  if (p.vec == 0)
+    snprintf(buf, len, "%s_long_cta%d", op, p.tpr);
+  else
+    snprintf(buf, len, "%s_vec%d%s_tpr%d_ch%d%s", op, p.vec, p.edge ? "_edge" : "", p.tpr, p.ch, p.stream ? "_stream" : "");
 }
 
 }  // namespace dtas

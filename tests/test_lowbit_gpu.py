@@ -111,6 +111,40 @@ def test_norm_without_residual_and_in_place(cuda_device, h):
     assert_fp16_close(x, y, y.abs().max() * FP32)
 
 
+@pytest.mark.parametrize("op,m,h,in_dtype", [("norm", 40001, 64, F16), ("norm", 5003, 1000, F16), ("norm", 900, 4104, F16),
+                                             ("norm", 300, 16384, F16), ("quantize", 12001, 136, F16),
+                                             ("quantize", 12001, 1024, F32), ("quantize", 20003, 8, F16)])
+def test_more_rows_than_fit_at_once(cuda_device, op, m, h, in_dtype):
+    assert _abi.variant_of("add_rms_norm" if op == "norm" else op, m, h).endswith("_stream")
+    x, res = randn(m, h, seed=m).to(in_dtype), randn(m, h, seed=m + 1, scale=2).to(in_dtype)
+    x[m // 2], res[m // 2] = 0, 0
+    x[m - 1, h - 1] = math.nan
+    w = (1 + randn(h, seed=2, scale=0.1)).to(F16)
+    fine = torch.arange(m - 1, device="cuda")
+    for out_dtype in (I8, E4M3) + ((F16,) if op == "norm" else ()):
+        out = torch.empty(m, h, dtype=out_dtype, device="cuda")
+        scale = torch.full((m,), 7.0, device="cuda")
+        if op == "quantize":
+            y = x.double()
+            ops.quantize(x, out, scale)
+        else:
+            hh, y = norm_of(x, res, w, 1e-6)
+            stream = res.clone()
+            ops.add_rms_norm(x, stream, w, out, res_out=stream, scale=scale)      # the residual stream updated in place
+            assert_h(stream[fine], hh[fine])
+            plain = torch.empty_like(out)                                          # neither a residual nor its sum
+            ops.add_rms_norm(x, None, w, plain, scale=torch.empty_like(scale))
+            one = torch.empty_like(out)
+            ops.add_rms_norm(x, torch.zeros_like(x), w, one, scale=torch.empty_like(scale))
+            assert torch.equal(plain.view(torch.uint8), one.view(torch.uint8))
+        if out_dtype == F16:
+            assert_fp16_close(out[fine], y[fine], y[fine].abs().max() * FP32)
+            assert torch.isnan(out[m - 1]).all()
+        else:
+            assert_rows8(out[fine], scale[fine], y[fine])
+            assert scale[m // 2] == 0 and torch.isnan(scale[m - 1])
+
+
 @pytest.mark.parametrize("in_dtype,out_dtype", [(F16, I8), (F16, E4M3), (F32, I8), (F32, E4M3)])
 @pytest.mark.parametrize("h", [64, 65, 40000])
 def test_rows_of_zeros_infinities_and_tiny_values(cuda_device, h, in_dtype, out_dtype):
