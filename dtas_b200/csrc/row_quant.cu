@@ -18,9 +18,11 @@
 // rounded up to whole warps and not to a power of two, so that 11008 columns take 352 threads x 4 chunks
 // and none idles.  Bound: HBM; every element is read once and written once.
 // Rows of a length that is no multiple of eight start anywhere inside a 16-byte vector, but at the same place in
-// every operand (EDGE): chunks are cut where the flat index is a multiple of eight, and only the first and the last
-// of a row, which it shares with its neighbours, go element by element ([8192, 4097] to e4m3 143 us element by
-// element throughout).
+// every operand (EDGE): chunks are cut where the flat index is a multiple of eight, loads take whole vectors, and of the
+// results only the first and the last chunk of a row, which it shares with its neighbours, go element by element.
+// Where the rows fill the device several times over, CTAs stay and take rows in turn (row_quant_stream_kernel).
+// Measured (HBM 6.57 TB/s): add_rms_norm fp16 to e4m3 [8192, 4096] 39.8 us, 5.9 TB/s; fp32 [4096, 4096] 33.3 us, 6.5 TB/s;
+// [1, 4096] 1.9 us; quantize to e4m3 [2048, 11008] 14.4 us, 4.7 TB/s; [8192, 4096] 17.5 us, 5.75 TB/s.
 #include <cuda_fp8.h>
 
 #include <atomic>
@@ -32,8 +34,9 @@ namespace {
 
 enum { Q_NORM = 0, Q_QUANT = 1 };
 constexpr int kMaxThreads = 1024;
-// Threads a CTA may have: what leaves a thread the registers for its chunks.
-constexpr int max_threads(int vec, int ch) { return vec * ch > 16 ? 512 : kMaxThreads; }
+// Threads a CTA may have: what leaves a thread the registers for its chunks, and one warp more than a row of 16384 elements
+// needs, for the one that starts inside a vector.
+constexpr int max_threads(int vec, int ch) { return vec * ch > 16 ? 544 : kMaxThreads; }
 
 struct RowArgs {
   const void* x;
@@ -66,27 +69,6 @@ __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_f32(float v) { return v; }
 
 // VEC consecutive elements of a row; VEC = 8 needs 16-byte aligned rows (32-byte pairs for fp32).
-template <int VEC, typename T>
-__device__ __forceinline__ void load_vec(const T* p, float* v) {
-  if constexpr (VEC == 8 && sizeof(T) == 2) {
-    const uint4 r = __ldcs(reinterpret_cast<const uint4*>(p));
-    const __half2* h = reinterpret_cast<const __half2*>(&r);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(h[i]);
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
-    }
-  } else if constexpr (VEC == 8) {
-    const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = to_f32(p[i]);
-  }
-}
-
 template <int VEC>
 __device__ __forceinline__ void store_vec(__half* p, const float* v) {
   if constexpr (VEC == 8) {
@@ -132,24 +114,55 @@ __device__ __forceinline__ void store_q(OutT* p, const float* v) {
 }
 
 // VEC weights as loaded.  They go through the read-only path: stores of the residual cannot alias them, so all of them are
-// under way with the rows instead of one behind each store.
+// under way with the rows instead of one behind each store.  A row that starts `lead` elements inside a vector needs eight
+// weights out of two vectors, moved together by whole words and then by half a word.
 template <int VEC, bool EDGE>
 struct Weights {
   static constexpr int kN = VEC == 8 ? 4 : VEC;
   uint32_t r[kN];
-  __device__ __forceinline__ void load(const __half* p, int e, int n) {
-    const unsigned short* u = reinterpret_cast<const unsigned short*>(p);
+  // the vector of p's elements b .. b + 7 (b a multiple of eight), zeros for those that are not in 0 .. n - 1; `some`: the
+  // warp has a vector that is partly there
+  static __device__ __forceinline__ void vector_at(const __half* p, int b, int n, bool some, uint32_t* w) {
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (b >= 0 && b + 8 <= n) v = __ldg(reinterpret_cast<const uint4*>(p + b));
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    if (some && b >= 0 && b < n && b + 8 > n) {
+      const unsigned short* u = reinterpret_cast<const unsigned short*>(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = b + 2 * i < n ? __ldg(u + b + 2 * i) : 0u, hi = b + 2 * i + 1 < n ? __ldg(u + b + 2 * i + 1) : 0u;
+        w[i] = lo | (hi << 16);
+      }
+    }
+  }
+  __device__ __forceinline__ void load(const __half* p, int e, int lead, int n) {
+    bool some = false;
+    if constexpr (EDGE) some = __any_sync(0xffffffffu, e + lead - 8 < n && e + lead + 8 > n);
+    if (e >= n) return;
     if constexpr (VEC == 8 && !EDGE) {
       const uint4 v = __ldg(reinterpret_cast<const uint4*>(p + e));
       r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w;
     } else if constexpr (VEC == 8) {
+      uint32_t w[8];
+      vector_at(p, lead ? e + lead - 8 : -8, n, some, w);
+      vector_at(p, e + lead, n, some, w + 4);
+      const int by = 8 - lead;
+      if (by & 8) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = e + 2 * i;
-        const uint32_t lo = j >= 0 && j < n ? __ldg(u + j) : 0u, hi = j + 1 >= 0 && j + 1 < n ? __ldg(u + j + 1) : 0u;
-        r[i] = lo | (hi << 16);
+        for (int i = 0; i < 4; ++i) w[i] = w[i + 4];
       }
+      if (by & 4) {
+#pragma unroll
+        for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+      }
+      if (by & 2) {
+#pragma unroll
+        for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = by & 1 ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
     } else {
+      const unsigned short* u = reinterpret_cast<const unsigned short*>(p);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) r[i] = __ldg(u + e + i);
     }
@@ -194,23 +207,78 @@ __device__ __forceinline__ void row_reduce(float& sum, float& top, float2* ex) {
   }
 }
 
-// A chunk of a row whose first element is e: whole, or (EDGE) the part of it that is the row's.
-template <int VEC, bool EDGE>
-__device__ __forceinline__ bool whole(int e, int n) {
-  return !EDGE || (e >= 0 && e + VEC <= n);
-}
-template <int VEC, bool EDGE, typename T>
-__device__ __forceinline__ void load_chunk(const T* row, int e, int n, float* v) {
-  if (whole<VEC, EDGE>(e, n)) {
-    load_vec<VEC>(row + e, v);
-  } else {
+// Sixteen-byte vectors of eight consecutive elements as loaded.
+template <typename T>
+struct Raw8 {
+  uint4 r[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = e + i >= 0 && e + i < n ? to_f32(row[e + i]) : 0.f;
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
   }
+  __device__ __forceinline__ void get(float* v) const {
+    const T* e = reinterpret_cast<const T*>(r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
+  }
+};
+
+// Which of a thread's chunks are partly outside the row (EDGE) for some thread of the warp, a bit each.  Two warps of a
+// row have one; the others branch around all that such chunks need.
+template <int VEC, int CH, bool EDGE>
+__device__ __forceinline__ unsigned edge_chunks(const int* at, int n) {
+  unsigned edges = 0;
+  if constexpr (EDGE) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+      if (__any_sync(0xffffffffu, at[c] < n && (at[c] < 0 || at[c] + VEC > n))) edges |= 1u << c;
+  }
+  return edges;
 }
-template <int VEC, bool EDGE, typename T>
-__device__ __forceinline__ void store_chunk(T* row, int e, int n, const float* v) {
-  if (whole<VEC, EDGE>(e, n)) {
+
+// A thread's chunks of a row, asked for at once and looked at later: nothing between the loads of a row and of its residual
+// waits for either.  A vector that is partly the row's is read whole all the same, for the rest of it is the rows' before
+// and behind, and only what the tensor ends in (`room` elements from the row's first) goes by its elements.
+template <int VEC, int CH, bool EDGE, typename T>
+struct RowChunks {
+  Raw8<T> raw[CH];
+  __device__ __forceinline__ void load(const T* row, const int* at, int n, int room) {
+    if constexpr (VEC == 8) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+        if (at[c] < n && (!EDGE || at[c] + 8 <= room)) raw[c].load(row + at[c]);
+    }
+  }
+  // chunk c, zeros where it lies outside the row
+  __device__ __forceinline__ void get(const T* row, int c, int at, int n, int room, unsigned edges, float* v) const {
+    if constexpr (VEC == 8) {
+      if (at < n) {
+        raw[c].get(v);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.f;
+      }
+      if (EDGE && (edges >> c & 1)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (at + i < 0 || at + i >= n) v[i] = 0.f;
+          else if (at + 8 > room) v[i] = to_f32(row[at + i]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = at < n ? to_f32(row[at + i]) : 0.f;
+    }
+  }
+};
+// The chunk whose first element is e back into the row; edge: some thread's is partly outside.
+template <int VEC, typename T>
+__device__ __forceinline__ void store_chunk(T* row, int e, int n, bool edge, const float* v) {
+  if (!edge) {
+    if (e < n) {
+      if constexpr (sizeof(T) == 1) store_q<VEC>(row + e, v);
+      else store_vec<VEC>(row + e, v);
+    }
+  } else if (e >= 0 && e + VEC <= n) {
     if constexpr (sizeof(T) == 1) store_q<VEC>(row + e, v);
     else store_vec<VEC>(row + e, v);
   } else {
@@ -241,8 +309,8 @@ __device__ __forceinline__ float quant_scale(float top, float r, float q) {
 
 // A row whose elements - for the norm, their sums with the residual - are in registers: its results.
 template <int OP, typename InT, typename OutT, int VEC, int CH, bool EDGE>
-__device__ __forceinline__ void finish_row(const RowArgs& a, int64_t row, bool live, int n, const int* at, float (*v)[VEC],
-                                           const Weights<VEC, EDGE>* wt, float2* ex) {
+__device__ __forceinline__ void finish_row(const RowArgs& a, int64_t row, bool live, int n, const int* at,
+                                           unsigned edges, float (*v)[VEC], const Weights<VEC, EDGE>* wt, float2* ex) {
   constexpr bool kNorm = OP == Q_NORM;
   constexpr bool k8 = sizeof(OutT) == 1;
   const int64_t off = row * a.n_cols;
@@ -252,8 +320,8 @@ __device__ __forceinline__ void finish_row(const RowArgs& a, int64_t row, bool l
     for (int c = 0; c < CH; ++c) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) sum = fmaf(v[c][i], v[c][i], sum);
+      if (a.res_out != nullptr) store_chunk<VEC>(static_cast<InT*>(a.res_out) + off, at[c], n, edges >> c & 1, v[c]);
       if (at[c] < n) {
-        if (a.res_out != nullptr) store_chunk<VEC, EDGE>(static_cast<InT*>(a.res_out) + off, at[c], n, v[c]);
         if constexpr (k8) {
 #pragma unroll
           for (int i = 0; i < VEC; ++i) v[c][i] *= wt[c].get(i);
@@ -277,22 +345,18 @@ __device__ __forceinline__ void finish_row(const RowArgs& a, int64_t row, bool l
     if (threadIdx.x == 0) a.scale[row] = quant_scale(top, r, OutTraits<OutT>::kQ);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      if (at[c] < n) {
-        float q[VEC];
+      float q[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) q[i] = (v[c][i] * qm.pre) * qm.mul;
-        store_chunk<VEC, EDGE>(y, at[c], n, q);
-      }
+      for (int i = 0; i < VEC; ++i) q[i] = (v[c][i] * qm.pre) * qm.mul;
+      store_chunk<VEC>(y, at[c], n, edges >> c & 1, q);
     }
   } else {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      if (at[c] < n) {
-        float o[VEC];
+      float o[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) o[i] = __fmul_rn(__fmul_rn(v[c][i], r), wt[c].get(i));
-        store_chunk<VEC, EDGE>(reinterpret_cast<__half*>(y), at[c], n, o);
-      }
+      for (int i = 0; i < VEC; ++i) o[i] = __fmul_rn(__fmul_rn(v[c][i], r), wt[c].get(i));
+      store_chunk<VEC>(reinterpret_cast<__half*>(y), at[c], n, edges >> c & 1, o);
     }
   }
 }
@@ -313,111 +377,95 @@ __global__ void __launch_bounds__(max_threads(VEC, CH)) row_quant_kernel(const R
 
   pdl_wait();
   pdl_launch_dependents();
-  float v[CH][VEC];
-#pragma unroll
-  for (int c = 0; c < CH; ++c) {
-    if (at[c] < n) {
-      load_chunk<VEC, EDGE>(x, at[c], n, v[c]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) v[c][i] = 0.f;
-    }
-  }
+  const unsigned edges = edge_chunks<VEC, CH, EDGE>(at, n);
+  const int64_t behind = a.m * a.n_cols - off;      // elements from the row's first to the tensor's last
+  const int room = behind < (1 << 30) ? (int)behind : 1 << 30;
+  const InT* res = kNorm && a.res != nullptr ? static_cast<const InT*>(a.res) + off : nullptr;
+  RowChunks<VEC, CH, EDGE, InT> rx, rr;
+  rx.load(x, at, n, room);
+  if (res != nullptr) rr.load(res, at, n, room);
   Weights<VEC, EDGE> wt[CH];
   if constexpr (kNorm) {
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
-      if (at[c] < n) wt[c].load(a.weight, at[c], n);
+    for (int c = 0; c < CH; ++c) wt[c].load(a.weight, at[c], lead, n);
   }
-  if constexpr (kNorm) {
-    if (a.res != nullptr) {
-      const InT* res = static_cast<const InT*>(a.res) + off;
+  float v[CH][VEC];
 #pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        if (at[c] < n) {
-          float t[VEC];
-          load_chunk<VEC, EDGE>(res, at[c], n, t);
+  for (int c = 0; c < CH; ++c) {
+    rx.get(x, c, at[c], n, room, edges, v[c]);
+    if (res != nullptr) {
+      float t[VEC];
+      rr.get(res, c, at[c], n, room, edges, t);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) v[c][i] += t[i];
-        }
-      }
+      for (int i = 0; i < VEC; ++i) v[c][i] += t[i];
     }
   }
-  finish_row<OP, InT, OutT, VEC, CH, EDGE>(a, row, live, n, at, v, wt, ex);
+  finish_row<OP, InT, OutT, VEC, CH, EDGE>(a, row, live, n, at, edges, v, wt, ex);
 }
 
-// Sixteen-byte vectors of eight consecutive elements as loaded.
-template <typename T>
-struct Raw8 {
-  uint4 r[sizeof(T) / 2];
-  __device__ __forceinline__ void load(const T* p) {
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
-  }
-  __device__ __forceinline__ void get(float* v) const {
-    const T* e = reinterpret_cast<const T*>(r);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
-  }
-};
-
 // Many rows: the CTAs that fit on the device take rows in turn, and a row's loads are under way while the one before
-// it is reduced and stored; the weights stay in registers.
-template <int OP, typename InT, typename OutT, int CH>
-__global__ void __launch_bounds__(512) row_quant_stream_kernel(const RowArgs a) {
+// it is reduced and stored.  The weights stay in registers, but for rows that start elsewhere inside a vector each time.
+template <int OP, typename InT, typename OutT, int CH, bool EDGE>
+__global__ void __launch_bounds__(EDGE ? max_threads(8, 4) : 512) row_quant_stream_kernel(const RowArgs a) {
   __shared__ float2 ex[2][kMaxThreads / 32];       // in turn: a row's exchange cannot meet the one before it
   constexpr bool kNorm = OP == Q_NORM;
-  const int n = (int)a.n_cols;
-  int at[CH];
+  struct Place {
+    int n, lead, room;
+    int64_t off;
+  };
+  auto place = [&](int64_t row) {
+    Place p;
+    p.n = row < a.m ? (int)a.n_cols : 0;
+    p.off = (row < a.m ? row : 0) * a.n_cols;
+    p.lead = EDGE ? (int)(p.off & 7) : 0;
+    const int64_t behind = a.m * a.n_cols - p.off;
+    p.room = behind < (1 << 30) ? (int)behind : 1 << 30;
+    return p;
+  };
+  auto at_of = [&](const Place& p, int* at) {
 #pragma unroll
-  for (int c = 0; c < CH; ++c) at[c] = (c * blockDim.x + threadIdx.x) * 8;
+    for (int c = 0; c < CH; ++c) at[c] = (c * blockDim.x + threadIdx.x) * 8 - p.lead;
+  };
   const int64_t step = (int64_t)gridDim.x * blockDim.y;
   int64_t first = (int64_t)blockIdx.x * blockDim.y;
+  const InT *xs = static_cast<const InT*>(a.x), *rs = kNorm ? static_cast<const InT*>(a.res) : nullptr;
 
   pdl_wait();
   pdl_launch_dependents();
-  Raw8<InT> x[CH], res[CH];
-  auto fetch = [&](int64_t row) {
-    if (row >= a.m) return;
-    const InT* px = static_cast<const InT*>(a.x) + row * a.n_cols;
-#pragma unroll
-    for (int c = 0; c < CH; ++c)
-      if (at[c] < n) x[c].load(px + at[c]);
-    if (kNorm && a.res != nullptr) {
-      const InT* pr = static_cast<const InT*>(a.res) + row * a.n_cols;
-#pragma unroll
-      for (int c = 0; c < CH; ++c)
-        if (at[c] < n) res[c].load(pr + at[c]);
-    }
+  RowChunks<8, CH, EDGE, InT> rx, rr;
+  auto fetch = [&](const Place& p) {
+    int at[CH];
+    at_of(p, at);
+    rx.load(xs + p.off, at, p.n, p.room);
+    if (rs != nullptr) rr.load(rs + p.off, at, p.n, p.room);
   };
-  fetch(first + threadIdx.y);
-  Weights<8, false> wt[CH];
-  if constexpr (kNorm) {
-#pragma unroll
-    for (int c = 0; c < CH; ++c)
-      if (at[c] < n) wt[c].load(a.weight, at[c], n);
-  }
+  Place p = place(first + threadIdx.y);
+  fetch(p);
+  int at[CH];
+  Weights<8, EDGE> wt[CH];
   for (int turn = 0; first < a.m; first += step, turn ^= 1) {
     const int64_t row = first + threadIdx.y;
-    const bool live = row < a.m;
+    at_of(p, at);
+    if (kNorm && (EDGE || first == (int64_t)blockIdx.x * blockDim.y)) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) wt[c].load(a.weight, at[c], p.lead, (int)a.n_cols);
+    }
+    const unsigned edges = edge_chunks<8, CH, EDGE>(at, p.n);
     float v[CH][8];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      if (live && at[c] < n) {
-        x[c].get(v[c]);
-        if (kNorm && a.res != nullptr) {
-          float t[8];
-          res[c].get(t);
+      rx.get(xs + p.off, c, at[c], p.n, p.room, edges, v[c]);
+      if (rs != nullptr) {
+        float t[8];
+        rr.get(rs + p.off, c, at[c], p.n, p.room, edges, t);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[c][i] += t[i];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[c][i] = 0.f;
+        for (int i = 0; i < 8; ++i) v[c][i] += t[i];
       }
     }
-    fetch(row + step);
-    finish_row<OP, InT, OutT, 8, CH, false>(a, row, live, live ? n : 0, at, v, wt, ex[turn]);
+    const Place next = place(row + step);
+    fetch(next);
+    finish_row<OP, InT, OutT, 8, CH, EDGE>(a, row, row < a.m, p.n, at, edges, v, wt, ex[turn]);
+    p = next;
   }
 }
 
@@ -493,10 +541,27 @@ inline RowPlan row_plan(int64_t m, int64_t n_cols, bool aligned, bool norm, bool
   }
   if (!aligned) {
     p.ch = chunks <= 256 * 4 ? 4 : 16;
+  } else if (p.edge && norm) {
+    // What rows that start inside a vector need besides leaves room for fewer threads, so a thread has two chunks or more
+    // sooner ([8192, 4097] fp16 to int8: 163 us with one, 71 with two, 113 with four; [255, 2561] 3.8, 4.0 and 7.1); from
+    // 4352 columns on fp16 rows go in turn ([8192, 8191] 149 us, a row per CTA 197; [1, 16383] 6.3 and 8.1) and fp32 rows
+    // take four ([8192, 8191] 183 us, with two 215; [255, 8191] 10.4 with two).
+    if (chunks <= 544) {
+      p.ch = m > 592 || chunks > 512 ? 2 : 1;
+    } else if (!wide && chunks <= 4 * 544) {
+      p.stream = true;
+      p.ch = chunks <= 2 * 544 ? 2 : 4;
+    } else {
+      p.ch = m > 592 ? 4 : 2;
+    }
+  } else if (p.edge) {
+    // [8192, 1025] to int8: two chunks 11.6 us, four 13.5; [8192, 4097] 32.8 and 29.7; [255, 11009] 5.8 and 4.2
+    p.ch = m <= 592 && chunks <= 1024 ? 1 : (chunks <= 160 ? 2 : 4);
   } else {
     p.ch = m <= 592 || norm ? 1 : (chunks <= 128 ? 2 : 4);
-    while (chunks > (int64_t)p.ch * max_threads(8, p.ch)) p.ch *= 2;
   }
+  if (aligned)
+    while (chunks > (int64_t)p.ch * max_threads(8, p.ch)) p.ch *= 2;
   // Rows in turn, four chunks to a thread (as many as leave it whole warps): fp16 norms of enough elements to fill the
   // device a few times over - [8192, 4096] to e4m3 49 us a row per CTA, 40 us in turn; [900, 4096] 8.0 and 7.5; [600, 16384]
   // 23.6 and 15.2; but [900, 1024] 3.3 and 3.6, and fp32 norms, whose rows in flight take twice the registers, 33 and 42
@@ -516,17 +581,17 @@ inline RowPlan row_plan(int64_t m, int64_t n_cols, bool aligned, bool norm, bool
   return p;
 }
 
-template <int OP, typename InT, typename OutT, int CH>
+template <int OP, typename InT, typename OutT, int CH, bool EDGE>
 int launch_stream(const RowPlan& p, const RowArgs& a, int sm_count, cudaStream_t st) {
   static std::atomic<int> per_sm[kMaxThreads / 32 + 1];      // CTAs of so many warps that an SM holds, once asked for
   const int threads = p.tpr * p.rows;
   int fit = per_sm[threads / 32].load(std::memory_order_relaxed);
   if (fit == 0) {
-    DTAS_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, row_quant_stream_kernel<OP, InT, OutT, CH>, threads, 0));
+    DTAS_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, (row_quant_stream_kernel<OP, InT, OutT, CH, EDGE>), threads, 0));
     per_sm[threads / 32].store(fit, std::memory_order_relaxed);
   }
   const int64_t groups = (a.m + p.rows - 1) / p.rows, most = (int64_t)sm_count * fit;
-  launch_kernel(row_quant_stream_kernel<OP, InT, OutT, CH>, (unsigned)(groups < most ? groups : most), dim3(p.tpr, p.rows), 0,
+  launch_kernel((row_quant_stream_kernel<OP, InT, OutT, CH, EDGE>), (unsigned)(groups < most ? groups : most), dim3(p.tpr, p.rows), 0,
                 st, a);
   return after_launch("row_quant_stream_kernel");
 }
@@ -542,10 +607,12 @@ int launch_typed(const RowPlan& p, const RowArgs& a, int sm_count, cudaStream_t 
   }
   if (p.stream) {
     if constexpr (OP == Q_NORM && sizeof(InT) == 2) {
-      if (p.ch == 1) return launch_stream<OP, InT, OutT, 1>(p, a, sm_count, st);
-      if (p.ch == 4) return launch_stream<OP, InT, OutT, 4>(p, a, sm_count, st);
+      if (p.edge && p.ch == 2) return launch_stream<OP, InT, OutT, 2, true>(p, a, sm_count, st);
+      if (p.edge) return launch_stream<OP, InT, OutT, 4, true>(p, a, sm_count, st);
+      if (p.ch == 1) return launch_stream<OP, InT, OutT, 1, false>(p, a, sm_count, st);
+      if (p.ch == 4) return launch_stream<OP, InT, OutT, 4, false>(p, a, sm_count, st);
     }
-    if constexpr (OP == Q_QUANT || sizeof(InT) == 2) return launch_stream<OP, InT, OutT, 2>(p, a, sm_count, st);
+    if constexpr (OP == Q_QUANT || sizeof(InT) == 2) return launch_stream<OP, InT, OutT, 2, false>(p, a, sm_count, st);
   }
 #define DTAS_ROWQ_CASE(V, C, E)                                                                    \
   if (p.vec == V && p.ch == C && p.edge == E) {                                                    \
@@ -571,8 +638,7 @@ int launch_out(const RowPlan& p, const RowArgs& a, int out_dtype, int sm_count, 
 
 template <int OP>
 int launch_in(const RowArgs& a, int in_dtype, int out_dtype, int sm_count, cudaStream_t st) {
-  // with rows that start inside a vector the weights are read one by one
-  bool aligned = aligned16(a.x) && aligned16(a.res) && aligned16(a.res_out) && (a.n_cols % 8 != 0 || aligned16(a.weight));
+  bool aligned = aligned16(a.x) && aligned16(a.res) && aligned16(a.res_out) && aligned16(a.weight);
   aligned = aligned && (reinterpret_cast<uintptr_t>(a.y) & (out_dtype == DTAS_F16 ? 15 : 7)) == 0;
   const RowPlan p = row_plan(a.m, a.n_cols, aligned, OP == Q_NORM, in_dtype == DTAS_F32);
   if (in_dtype == DTAS_F16) return launch_out<OP, __half>(p, a, out_dtype, sm_count, st);

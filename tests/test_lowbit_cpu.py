@@ -89,6 +89,7 @@ def test_variants_have_names(lib):
     assert _abi.variant_of("add_rms_norm", 8192, 4096) == "add_rms_norm_vec8_tpr128_ch4_stream"
     assert _abi.variant_of("add_rms_norm", 600, 1024) == "add_rms_norm_vec8_tpr128_ch1"
     assert _abi.variant_of("quantize", 8192, 1024) == "quantize_vec8_tpr64_ch2_stream"
+    assert _abi.variant_of("add_rms_norm", 4, 16383) == "add_rms_norm_vec8_edge_tpr544_ch4_stream"
     assert _abi.variant_of("quantize", 1, 101) == "quantize_vec8_edge_tpr32_ch1"
     assert _abi.variant_of("add_rms_norm", 2, 1 << 20).startswith("add_rms_norm_long")
     assert "mma_m8" in _abi.variant_of("gemv_w4", 1, 4096, 4096) and "scalar" in _abi.variant_of("gemv_w4", 1, 4096, 34)

@@ -112,7 +112,8 @@ def test_norm_without_residual_and_in_place(cuda_device, h):
 
 
 @pytest.mark.parametrize("op,m,h,in_dtype", [("norm", 40001, 64, F16), ("norm", 5003, 1000, F16), ("norm", 900, 4104, F16),
-                                             ("norm", 300, 16384, F16), ("quantize", 12001, 136, F16),
+                                             ("norm", 300, 16384, F16), ("norm", 1500, 8191, F16), ("norm", 601, 16383, F16),
+                                             ("norm", 1003, 4361, F16), ("quantize", 12001, 136, F16),
                                              ("quantize", 12001, 1024, F32), ("quantize", 20003, 8, F16)])
 def test_more_rows_than_fit_at_once(cuda_device, op, m, h, in_dtype):
     assert _abi.variant_of("add_rms_norm" if op == "norm" else op, m, h).endswith("_stream")
