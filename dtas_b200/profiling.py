@@ -122,4 +122,12 @@ def algorithmic(op, m, n, k=0):
         return {"bytes": 2 * n * k + 2 * k + 2 * n, "flops": 2 * n * k}
     if op == "gemm":
         return {"bytes": 2 * (m * k + n * k + m * n), "flops": 2 * m * n * k}
+    if op == "add_rms_norm":    # fp16 with a residual, to 8 bits: two reads, the sum and the rows with their scales
+        return {"bytes": 7 * m * n + 2 * n + 4 * m, "flops": 0}
+    if op == "quantize":        # fp16 to 8 bits
+        return {"bytes": 3 * m * n + 4 * m, "flops": 0}
+    if op == "gemv_w4":         # fp16 rows, groups of 128 with scales
+        return {"bytes": n * k // 2 + n * k // 64 + 2 * m * (k + n), "flops": 2 * m * n * k}
+    if op == "gemm_f8":
+        return {"bytes": m * k + n * k + 4 * (m + n) + 2 * m * n, "flops": 2 * m * n * k}
     raise ValueError(op)

@@ -15,7 +15,8 @@ from .profiling import algorithmic
 
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("--op", required=True, choices=["cast", "add", "copy", "rms_norm", "softmax", "gemv", "gemm"])
+    ap.add_argument("--op", required=True, choices=["cast", "add", "copy", "rms_norm", "softmax", "gemv", "gemm",
+                                                    "add_rms_norm", "quantize", "gemv_w4", "gemm_f8"])
     ap.add_argument("--m", type=int, default=1)
     ap.add_argument("--n", type=int, default=4096)
     ap.add_argument("--k", type=int, default=4096)
@@ -43,6 +44,24 @@ def main():
         x, w = torch.randn(1, k, device=dev, dtype=f16), torch.randn(n, k, device=dev, dtype=f16) * 0.02
         y = torch.empty(1, n, device=dev, dtype=f16)
         fn = lambda: ops.gemv(x, w, y)  # noqa: E731
+    elif a.op in ("add_rms_norm", "quantize"):
+        x = torch.randn(m, n, device=dev, dtype=f16)
+        q, s = torch.empty(m, n, device=dev, dtype=torch.float8_e4m3fn), torch.empty(m, device=dev)
+        if a.op == "quantize":
+            fn = lambda: ops.quantize(x, q, s)  # noqa: E731
+        else:
+            w, res, h = torch.ones(n, device=dev, dtype=f16), torch.randn_like(x), torch.empty_like(x)
+            fn = lambda: ops.add_rms_norm(x, res, w, q, res_out=h, scale=s)  # noqa: E731
+    elif a.op == "gemv_w4":
+        x = torch.randn(m, k, device=dev, dtype=f16)
+        w = torch.randint(0, 256, (n, k // 2), device=dev, dtype=torch.uint8)
+        s, y = torch.full((n, k // 128), 0.01, device=dev, dtype=f16), torch.empty(m, n, device=dev, dtype=f16)
+        fn = lambda: ops.gemv_w4(x, w, s, y)  # noqa: E731
+    elif a.op == "gemm_f8":
+        x, w = (torch.randn(r, k, device=dev).clamp(-3, 3).to(torch.float8_e4m3fn) for r in (m, n))
+        xs, ws = torch.ones(m, device=dev), torch.full((n,), 0.02, device=dev)
+        y = torch.empty(m, n, device=dev, dtype=f16)
+        fn = lambda: ops.gemm_nt_f8(x, w, xs, ws, y)  # noqa: E731
     else:
         _abi.check(_abi.lib().dtas_gemm_set_override(a.bn, a.split_k))
         x, w = torch.randn(m, k, device=dev, dtype=f16), torch.randn(n, k, device=dev, dtype=f16) * 0.02
@@ -65,7 +84,7 @@ def main():
     torch.cuda.synchronize()
     ops.poll_status(0)
     us = 1e3 * e0.elapsed_time(e1) / a.iters
-    alg = algorithmic(a.op, m, n, k if a.op in ("gemv", "gemm") else 0)
+    alg = algorithmic(a.op, m, n, k if a.op.startswith("ge") else 0)
     print(f"{a.op} m={m} n={n} k={k}: {_abi.variant_of(a.op, m, n, k, 0)}  {us:.2f} us/launch  "
           f"{alg['bytes'] / us / 1e3:.0f} GB/s  {alg['flops'] / us / 1e6:.1f} TFLOP/s")
 

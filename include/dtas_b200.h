@@ -135,8 +135,9 @@ int dtas_gemv_fused(const void* x, const void* w, const void* bias, const void* 
  *   W[n, k] = w_scale[n, k / group] * (code - w_zero[n, k / group]).  w holds two 4-bit codes to a byte, [n, k / 2],
  *   the even k in the low half; w_scale fp16 and w_zero uint8 [n, k / group]; w_zero NULL stands for 8 everywhere.
  *   x is DTAS_F16 with x_scale NULL, or DTAS_I8 / DTAS_E4M3 with an fp32 scale per row.  k must be even and
- *   a multiple of group.  Tail operands as in dtas_gemv_fused, with rows of n elements.  Groups and k that are
- *   multiples of 32 with 16-byte aligned x and w take the fast kernel, everything else a scalar one.
+ *   a multiple of group.  Tail operands as in dtas_gemv_fused, with rows of n elements.  k a multiple of 32 in groups of
+ *   32, 64 or a multiple of 128 with 16-byte aligned x, w, w_scale and w_zero takes the tensor-core kernel, anything
+ *   else a scalar one (some ten to a hundred times slower).
  * dtas_gemm_nt_f8: y = act(x_scale[m] w_scale[n] (x . w^T) + bias) + res1 + res2 of e4m3 operands x [m, k] and
  *   w [n, k] with fp32 scales per row of each, on the tcgen05 tensor cores; ldy, ldr and the tail as in
  *   dtas_gemm_nt_fused.  k a multiple of 16 and 16-byte aligned operands; else a scalar kernel.  Its
