@@ -1282,8 +1282,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairMaxThreads, 1)
       __half my_bias[2] = {__half(0.f), __half(0.f)};
       if constexpr (F8) {
         // The main loop of an e4m3 tile is half as long as an fp16 tile's, too short to hide a trip to L2 for every 32
-        // columns' scales and bias behind it (1000 x 10240 x 2560 with bias: 39.5 us so, 30.5 this way, 27.3 without bias): a thread fetches its columns' (one of eight warps, two of four) while
-        // the tile is computed, and they wait in shared memory for the arithmetic.
+        // columns' scales and bias behind it (1000 x 10240 x 2560 with bias: 39.5 us so, 30.5 this way, 27.3 without
+        // bias): a thread fetches its columns' (one of eight warps, two of four) while the tile is computed, and they
+        // wait in shared memory for the arithmetic.
         const int r = mt * 2 * BM + (int)rank * BM + quarter * 32 + lane;
         if (r < a.m) row_scale = a.epi.sx[r];
 #pragma unroll
@@ -1502,9 +1503,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairMaxThreads, 1)
           }
         }
       } else if (F8) {
-        // Residuals beside e4m3 operands ([1000, 10240] x 2560: 45 us, 58 with each thread reading its row): blocks of 64 columns of the first come in by rows (a load instruction covers
-        // four 128-byte lines, not 32 pieces of 16 bytes), a block ahead, and are laid out in the stage, where the
-        // results then take their places.  Ragged and unaligned ones are read in place.
+        // Residuals beside e4m3 operands ([1000, 10240] x 2560: 45 us, 58 with each thread reading its row): blocks of
+        // 64 columns of the first come in by rows (a load instruction covers four 128-byte lines, not 32 pieces of 16
+        // bytes), a block ahead, and are laid out in the stage, where the results then take their places.  Ragged and
+        // unaligned ones are read in place.
         const bool by_rows = DTAS_PAIR_STAGED_STORE && a.epi.vec_res && a.vec_store && !a.epi.out_f32 &&
                              col_base + c_end * 32 <= a.n && (c_end & 1) == 0;
         const int row0 = mt * 2 * BM + (int)rank * BM + quarter * 32;
