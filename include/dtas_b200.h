@@ -127,7 +127,7 @@ int dtas_gemv_fused(const void* x, const void* w, const void* bias, const void* 
  *   x, res [m, n_cols] of in_dtype (DTAS_F16 or DTAS_F32); res may be NULL (h = x).  res_out, optional, receives
  *   h in in_dtype and may be x or res itself; weight fp16 [n_cols].  The norm is taken of h before that
  *   rounding.  y is out_dtype: DTAS_F16, or DTAS_I8 / DTAS_E4M3 with one fp32 scale per row in scale [m]:
- *   scale = max|y| / Q, y = round(value / scale), Q = 127 or 448, ties to even.  A row of zeros gets scale 0
+ *   scale = max|y| / Q, y = round(value * Q / max|y|), Q = 127 or 448, ties to even.  A row of zeros gets scale 0
  *   (y = 0); a row whose values hold an infinity or a NaN gets a NaN scale.  scale is not used for fp16.
  * dtas_quantize: the same 8-bit form of the rows of x itself; also how a weight matrix [n, k] is brought to
  *   8 bits with a scale per row for dtas_gemm_nt_f8.

@@ -1,0 +1,86 @@
+"""The low-bit path on the GPU where a result is known exactly, and at its edges: values halfway between two 8-bit ones."""
+import math
+
+import pytest
+import torch
+
+from dtas_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+F16, F32, I8, E4M3 = torch.float16, torch.float32, torch.int8, torch.float8_e4m3fn
+Q = {I8: 127.0, E4M3: 448.0}
+
+
+# ---- values halfway between two 8-bit ones -----------------------------------------------------------
+def halfway(dtype):
+    """Every number halfway between neighbours of dtype, both signs, fp64."""
+    if dtype == I8:
+        t = torch.arange(0, 127, dtype=torch.float64) + 0.5
+    else:
+        steps = [torch.arange(0, 8, dtype=torch.float64) * 2.0 ** -9 + 2.0 ** -10]
+        steps += [(torch.arange(8, 16, dtype=torch.float64) + 0.5) * 2.0 ** (e - 3) for e in range(-6, 9)]
+        t = torch.cat(steps)
+        t = t[t < 448]
+    return torch.cat((t, -t))
+
+
+def rows_of_halves(dtype, in_dtype, width):
+    """Rows v with a maximum top such that v Q / top is halfway between two 8-bit values, all of it exact: with an odd s,
+    v = t s / unit and top = Q s / unit for the halfway numbers t.  -> v, the t, both fp64 [rows, width]"""
+    t = halfway(dtype)
+    unit = 64.0 if dtype == E4M3 else 1.0
+    if in_dtype == F16:        # s times the bits of t, 5 or 8 of them, within the 11 of fp16
+        factors = range(1, 64, 2) if dtype == E4M3 else range(1, 8, 2)
+        factors = [float(s) for s in factors]
+    else:                      # 24 bits, over the range of fp32 exponents as well
+        factors = [float(2 * s + 1) * 2.0 ** e for s, e in zip(range(0, 30000, 311), [0, -3, 20, -60, 70, -100, 95, -115, 0, 0] * 10)]
+    v = torch.zeros(len(factors), width, dtype=torch.float64)
+    want = torch.zeros_like(v)
+    for i, s in enumerate(factors):
+        v[i, 0], want[i, 0] = Q[dtype] * s / unit, Q[dtype]
+        v[i, 1:1 + len(t)], want[i, 1:1 + len(t)] = t * s / unit, t
+    assert torch.equal(v.to(in_dtype).double(), v)
+    return v, want
+
+
+def to_even(t, dtype):
+    return t.round().to(I8) if dtype == I8 else t.to(F32).to(E4M3)      # t is an fp32 number: one rounding, to even
+
+
+@pytest.mark.parametrize("width", [264, 271, 40001])
+@pytest.mark.parametrize("in_dtype", [F16, F32])
+@pytest.mark.parametrize("dtype", [I8, E4M3])
+def test_halves_go_to_the_even_value(cuda_device, dtype, in_dtype, width):
+    v, t = rows_of_halves(dtype, in_dtype, width)
+    m, want = len(v), to_even(t, dtype).cuda()
+    buf = torch.zeros(m * width + 8, dtype=in_dtype, device="cuda")
+    for off in (0, 1):                                                       # 16-byte vectors, and one element at a time
+        x = buf[off:off + m * width].view(m, width)
+        x.copy_(v)
+        q, scale = torch.empty(m, width, dtype=dtype, device="cuda"), torch.empty(m, device="cuda")
+        ops.quantize(x, q, scale)
+        assert torch.equal(q.float(), want.float())
+        top = v.abs().amax(-1).cuda()
+        assert ((scale.double() - top / Q[dtype]).abs() <= top / Q[dtype] * 2.0 ** -24 + 2.0 ** -150).all()
+        # through the norm, weights of one: its factor cancels, and the sum of two halves of v is v
+        weight = torch.ones(width, dtype=F16, device="cuda")
+        sane = (top < 1e18) & (top > 1e-15)                                  # squares within fp32
+        ops.add_rms_norm(x, None, weight, q, scale=scale)
+        assert torch.equal(q.float()[sane], want.float()[sane])
+        if in_dtype == F32:
+            half = x / 2
+            ops.add_rms_norm(half, half, weight, q, scale=scale)
+            assert torch.equal(q.float()[sane], want.float()[sane])
+
+
+@pytest.mark.parametrize("dtype", [I8, E4M3])
+def test_rows_of_fp16_numbers_are_rounded_once(cuda_device, dtype):
+    """Of fp16 rows the exact quotient is known: v Q is a number of at most 18 bits, and a quotient that is not halfway
+    is further from there than 2^-19 of itself."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = (torch.randn(300, 4096, generator=g, device="cuda") * 8).to(F16)
+    q, scale = torch.empty(300, 4096, dtype=dtype, device="cuda"), torch.empty(300, device="cuda")
+    ops.quantize(x, q, scale)
+    y = x.double() * Q[dtype] / x.double().abs().amax(-1, keepdim=True)
+    assert torch.equal(q.float(), (y.round() if dtype == I8 else y.to(F32).to(E4M3)).float())
