@@ -170,9 +170,18 @@ def _tail_args(name, out, n, rows, bias, res1, res2, act):
     for r in (res1, res2):
         if r is None:
             continue
-        if r.dtype != torch.float16 or r.numel() != rows * n or r.stride(-1) != 1:
-            raise _abi.DtasError(_abi.EINVAL, f"{name}: residuals must be fp16 [m, N] with unit inner stride")
-        ld = max(int(r.stride(-2)), n) if r.dim() >= 2 else n
+        # rows of n elements, one behind the other, or [m, N] with rows further apart: nothing else may give the kernel a row
+        # stride, for it would read rows where there are none (a row stride of 0, [N, m])
+        shape = tuple(r.shape)
+        if r.is_contiguous() and r.numel() == rows * n and (rows == 1 or shape[-1] == n):
+            ld = n
+        elif shape in ((rows, n), (1, rows, n)) and (n == 1 or r.stride(-1) == 1) and r.stride(-2) >= n:
+            ld = int(r.stride(-2))
+        else:
+            ld = 0
+        if r.dtype != torch.float16 or ld == 0:
+            raise _abi.DtasError(_abi.EINVAL, f"{name}: residuals must be fp16 [m, N] with unit inner stride and rows that do not "
+                                              f"overlap, got {r.dtype} {shape} with strides {tuple(r.stride())}")
         if ldr and ld != ldr and rows > 1:
             raise _abi.DtasError(_abi.EINVAL, f"{name}: both residuals must have the same row stride")
         ldr = ld

@@ -1,0 +1,52 @@
+"""The low-bit path's edges without a GPU: which residuals its products take, with which row stride."""
+import pytest
+import torch
+
+from dtas_b200 import _abi, ops
+
+F16 = torch.float16
+
+
+def row_stride(rows, n, *residuals):
+    """The row stride with which a product of `rows` rows of n reads these residuals."""
+    out = torch.empty(rows, n, dtype=F16)
+    return ops._tail_args("gemm_f8", out, n, rows, None, residuals[0], residuals[1] if len(residuals) > 1 else None, None)[2]
+
+
+def z(*shape):
+    return torch.zeros(*shape, dtype=F16)
+
+
+@pytest.mark.parametrize("residual,stride", [
+    (z(4, 8), 8), (z(1, 4, 8), 8), (z(2, 2, 8), 8), (z(4, 20)[:, 4:12], 20), (z(1, 4, 20)[:, :, 4:12], 20), (z(8, 8)[::2], 16)])
+def test_residual_rows(residual, stride):
+    assert row_stride(4, 8, residual) == stride
+    assert row_stride(4, 8, residual, residual) == stride
+
+
+@pytest.mark.parametrize("residual", [z(8), z(1, 8), z(1, 1, 8), z(8, 1)])
+def test_residual_of_one_row(residual):
+    assert row_stride(1, 8, residual) == 8
+
+
+def test_residual_of_one_column():
+    assert row_stride(4, 1, z(4, 1)) == 1 and row_stride(4, 1, z(4, 6)[:, 2:3]) == 6
+
+
+@pytest.mark.parametrize("residual", [
+    z(8).expand(4, 8), z(1, 8).expand(4, 8), z(1, 1, 8).expand(1, 4, 8),      # a row stride of 0
+    z(8, 4), z(16, 2), z(32), z(1, 8, 4),                                    # as many elements in another shape
+    z(8, 4).t(), z(4, 16)[:, ::2],                                           # an inner stride
+    z(2, 4, 8)[:, ::2], z(2, 2, 20)[:, :, :8],                               # rows that no one stride describes
+    z(100).as_strided((4, 8), (4, 1)),                                       # rows that overlap
+    z(4, 8).float()])
+def test_residuals_that_a_row_stride_does_not_describe_are_refused(residual):
+    for args in ((residual,), (z(4, 8), residual)):
+        with pytest.raises(_abi.DtasError) as e:
+            row_stride(4, 8, *args)
+        assert e.value.code == _abi.EINVAL
+
+
+def test_two_residuals_share_a_row_stride():
+    with pytest.raises(_abi.DtasError):
+        row_stride(4, 8, z(4, 8), z(4, 20)[:, :8])

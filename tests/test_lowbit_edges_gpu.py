@@ -1,10 +1,9 @@
-"""The low-bit path on the GPU where a result is known exactly, and at its edges: values halfway between two 8-bit ones."""
-import math
-
+"""The low-bit path on the GPU where a result is known exactly, and at its edges: values halfway between two 8-bit ones, residuals
+of other shapes and strides."""
 import pytest
 import torch
 
-from dtas_b200 import ops
+from dtas_b200 import _abi, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -84,3 +83,19 @@ def test_rows_of_fp16_numbers_are_rounded_once(cuda_device, dtype):
     ops.quantize(x, q, scale)
     y = x.double() * Q[dtype] / x.double().abs().amax(-1, keepdim=True)
     assert torch.equal(q.float(), (y.round() if dtype == I8 else y.to(F32).to(E4M3)).float())
+
+
+# ---- residuals of other shapes and strides -----------------------------------------------------------
+def test_residuals_of_other_shapes_are_refused(cuda_device):
+    m, n, k = 12, 24, 64
+    z = lambda *shape, dt=F16: torch.zeros(*shape, dtype=dt, device="cuda")  # noqa: E731
+    x, w, x8, w8 = z(m, k), z(n, k), z(m, k, dt=F32).to(E4M3), z(n, k, dt=F32).to(E4M3)
+    codes, scales = z(n, k // 2, dt=torch.uint8), z(n, 2)
+    out = torch.full((m, n), 3.0, dtype=F16, device="cuda")
+    for r in (z(n, m), z(n).expand(m, n), z(1, n).expand(m, n), z(2 * m, n // 2), z(m * n), z(m, n).float(), z(m - 1, n)):
+        for kw in ({"res1": r}, {"res1": z(m, n), "res2": r}):
+            for call in (lambda: ops.gemm_nt_f8(x8, w8, z(m, dt=F32), z(n, dt=F32), out, **kw), lambda: ops.gemv_w4(x, codes, scales, out, **kw),
+                         lambda: ops.gemm_nt(x, w, out, **kw)):
+                with pytest.raises(_abi.DtasError):
+                    call()
+    assert (out == 3.0).all()
