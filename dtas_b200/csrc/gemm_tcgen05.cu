@@ -198,18 +198,18 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld_wait() {
+// Waits for the loads issued before it and makes later uses of the words `r` depend on the wait.  The load's asm hands its
+// destination registers over when it is issued, and neither a volatile asm nor its memory clobber keeps arithmetic on
+// registers alone (a scale or a residual fetched earlier) from being scheduled ahead of a wait that does not name them.
+template <int N>
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[N]) {
+  static_assert(N == 16 || N == 32, "what one load brings");
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-// After a wait: makes later uses of the loaded registers depend on the wait.  Where a load is issued well
-// before its wait (to be in flight during other work), nothing else keeps arithmetic on its
-// destination registers from being scheduled ahead of the wait.
-__device__ __forceinline__ void tmem_ld_landed(uint32_t* r) {
-  asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                    "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
-  asm volatile("" : "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
-                    "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
-                    "+r"(r[30]), "+r"(r[31]));
+#pragma unroll
+  for (int h = 0; h < N; h += 16)
+    asm volatile("" : "+r"(r[h + 0]), "+r"(r[h + 1]), "+r"(r[h + 2]), "+r"(r[h + 3]), "+r"(r[h + 4]), "+r"(r[h + 5]), "+r"(r[h + 6]),
+                      "+r"(r[h + 7]), "+r"(r[h + 8]), "+r"(r[h + 9]), "+r"(r[h + 10]), "+r"(r[h + 11]), "+r"(r[h + 12]),
+                      "+r"(r[h + 13]), "+r"(r[h + 14]), "+r"(r[h + 15]));
 }
 __device__ __forceinline__ void epilogue_bar_sync() {
   asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueThreads) : "memory");
@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
               for (int cc = c; cc < c + kBlk; ++cc) {
                 uint32_t r[32];
                 tmem_ld32(t_addr + cc * 32, r);
-                tmem_ld_wait();
+                tmem_ld_wait(r);
                 const int col0 = col_base + cc * 32;
                 if (row_ok && col0 < a.n) epi_store_row32_plain(a.epi.bias, yrow, a.vec_store, col0, a.n, r);
               }
@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             for (int cc = 0; cc < kBlk; ++cc) {
               uint32_t r[32];
               tmem_ld32(t_addr + (c + cc) * 32, r);
-              tmem_ld_wait();
+              tmem_ld_wait(r);
               float f[32];
 #pragma unroll
               for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(r[j]);
@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           const ResChunk r_now = r_next;
           r_next = r_after;
           if (row_ok && c + 2 < BN / 32 && epi_can_prefetch(a.epi, col0 + 64, a.n)) epi_prefetch_res32(a.epi, row, col0 + 64, r_after);
-          tmem_ld_wait();
+          tmem_ld_wait(r);
           if (row_ok && col0 < a.n) {
             float f[32];
 #pragma unroll
@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         for (int c = 0; c < BN / 32; ++c) {
           uint32_t r[32];
           tmem_ld32(t_addr + c * 32, r);
-          tmem_ld_wait();
+          tmem_ld_wait(r);
           if (row_ok && col_base + c * 32 < a.n) {
 #pragma unroll
             for (int q = 0; q < 8; ++q)
@@ -828,7 +828,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           uint32_t r[kChunk];
           if constexpr (kChunk == 16) tmem_ld16(t_addr + c * kChunk, r);
           else tmem_ld32(t_addr + c * kChunk, r);
-          tmem_ld_wait();
+          tmem_ld_wait(r);
           if (col_ok) {
             float f[kChunk];
 #pragma unroll
@@ -852,7 +852,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           uint32_t r[kChunk];
           if constexpr (kChunk == 16) tmem_ld16(t_addr + c * kChunk, r);
           else tmem_ld32(t_addr + c * kChunk, r);
-          tmem_ld_wait();
+          tmem_ld_wait(r);
 #pragma unroll
           for (int q = 0; q < kChunk / 4; ++q) {
             const int g = c * (kChunk / 4) + q;
@@ -1336,7 +1336,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairMaxThreads, 1)
         for (int c = c_begin; c < c_end; ++c) {
           uint32_t r[32];
           tmem_ld32(t_addr + c * 32, r);
-          tmem_ld_wait();
+          tmem_ld_wait(r);
           if (row_ok && col_base + c * 32 < a.n) {
 #pragma unroll
             for (int q = 0; q < 8; ++q)
@@ -1389,10 +1389,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairMaxThreads, 1)
               }
               if (own0) {                    // the same for the whole warp
                 tmem_ld32(t_addr + c * 32, v0);
-                tmem_ld_wait();
+                tmem_ld_wait(v0);
               } else if (own1) {
                 tmem_ld32(t_addr + c * 32, v1);
-                tmem_ld_wait();
+                tmem_ld_wait(v1);
               }
 #pragma unroll
               for (int j = 0; j < 32; ++j) f[j] += __uint_as_float(v0[j]);
@@ -1428,7 +1428,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairMaxThreads, 1)
             for (int cc = c; cc < min(c + 4, c_end); ++cc) {
               uint32_t r[32];
               tmem_ld32(t_addr + cc * 32, r);
-              tmem_ld_wait();
+              tmem_ld_wait(r);
               const int col0 = col_base + cc * 32;
               if (row_ok && col0 < a.n) epi_store_row32_plain(a.epi.bias, yrow, a.vec_store, col0, a.n, r, &a.peers, (int64_t)row * a.ldy);
             }
@@ -1438,7 +1438,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairMaxThreads, 1)
           for (int cc = 0; cc < 4; ++cc) {
             uint32_t r[32];
             tmem_ld32(t_addr + (c + cc) * 32, r);
-            tmem_ld_wait();
+            tmem_ld_wait(r);
             if (a.epi.bias != nullptr) epi_add_bias32(a.epi.bias, colb + cc * 32, a.n, reinterpret_cast<float*>(r));
             float f[32];
 #pragma unroll
@@ -1486,20 +1486,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairMaxThreads, 1)
         // tensor memory while the current chunk is worked on (two sets of registers in turn).
         uint32_t ra[32], rb[32];
         tmem_ld32(t_addr + c_begin * 32, ra);
-        tmem_ld_wait();
-        tmem_ld_landed(ra);
+        tmem_ld_wait(ra);
 #pragma unroll 1
         for (int c = c_begin; c < c_end; c += 2) {        // c_begin is even: a pair of chunks is a staged block
           const bool second = c + 1 < c_end;
           if (second) tmem_ld32(t_addr + (c + 1) * 32, rb);
           finish_chunk(c, ra, nullptr);
-          tmem_ld_wait();
-          tmem_ld_landed(rb);
+          tmem_ld_wait(rb);
           if (second) {
             if (c + 2 < c_end) tmem_ld32(t_addr + (c + 2) * 32, ra);
             finish_chunk(c + 1, rb, nullptr);
-            tmem_ld_wait();
-            tmem_ld_landed(ra);
+            tmem_ld_wait(ra);
           }
         }
       } else if (F8) {
@@ -1542,7 +1539,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairMaxThreads, 1)
               for (int q = 0; q < 4; ++q) r_now.v[1][q] = s2[q];
             }
           }
-          tmem_ld_wait();
+          tmem_ld_wait(r);
           finish_chunk(c, r, by_rows ? &r_now : nullptr);
         }
       } else {
@@ -1559,7 +1556,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairMaxThreads, 1)
           const ResChunk r_now = r_next;
           r_next = r_after;
           if (row_ok && c + 2 < c_end && epi_can_prefetch(a.epi, col0 + 64, a.n)) epi_prefetch_res32(a.epi, row, col0 + 64, r_after);
-          tmem_ld_wait();
+          tmem_ld_wait(r);
           finish_chunk(c, r, epi_can_prefetch(a.epi, col0, a.n) ? &r_now : nullptr);
         }
       }
@@ -1722,7 +1719,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
         for (int c = 0; c < BN / 32; ++c) {
           uint32_t r[32];
           tmem_ld32(t_addr + c * 32, r);
-          tmem_ld_wait();
+          tmem_ld_wait(r);
 #pragma unroll
           for (int q = 0; q < 8; ++q)
             staging4[(c * 8 + q) * BM + r_in_tile] =
@@ -1740,7 +1737,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
         for (int c = 0; c < BN / 32; ++c) {
           uint32_t r[32];
           tmem_ld32(t_addr + c * 32, r);
-          tmem_ld_wait();
+          tmem_ld_wait(r);
           const int col0 = col_base + c * 32;
           if (row_ok && col0 < a.n) {
             float f[32];
@@ -1891,7 +1888,7 @@ __global__ void __cluster_dims__(S, 1, 1) __launch_bounds__(kGemmThreads, 1)
           uint32_t r[kChunk];
           if constexpr (kChunk == 16) tmem_ld16(t_addr + c * kChunk, r);
           else tmem_ld32(t_addr + c * kChunk, r);
-          tmem_ld_wait();
+          tmem_ld_wait(r);
 #pragma unroll
           for (int q = 0; q < kChunk / 4; ++q) {
             const int g = c * (kChunk / 4) + q;
@@ -1915,7 +1912,7 @@ __global__ void __cluster_dims__(S, 1, 1) __launch_bounds__(kGemmThreads, 1)
           uint32_t r[kChunk];
           if constexpr (kChunk == 16) tmem_ld16(t_addr + c * kChunk, r);
           else tmem_ld32(t_addr + c * kChunk, r);
-          tmem_ld_wait();
+          tmem_ld_wait(r);
           if (col_ok) {
             float f[kChunk];
 #pragma unroll

@@ -1,8 +1,13 @@
-"""The low-bit path's edges without a GPU: which residuals its products take, with which row stride."""
+"""The low-bit path's edges without a GPU: which residuals its products take, with which row stride, and the order of loads from
+tensor memory and of what uses them."""
+import os
+import re
+
 import pytest
 import torch
 
 from dtas_b200 import _abi, ops
+from dtas_b200.build import CSRC
 
 F16 = torch.float16
 
@@ -50,3 +55,15 @@ def test_residuals_that_a_row_stride_does_not_describe_are_refused(residual):
 def test_two_residuals_share_a_row_stride():
     with pytest.raises(_abi.DtasError):
         row_stride(4, 8, z(4, 8), z(4, 20)[:, :8])
+
+
+def test_every_wait_for_tensor_memory_names_its_registers():
+    """A tcgen05.ld's destination registers are the compiler's as soon as the load is issued: a wait that does not name
+    them does not order arithmetic on them."""
+    src = "".join(open(os.path.join(CSRC, f)).read() for f in sorted(os.listdir(CSRC)))
+    assert src.count("tcgen05.wait::ld") == 1 and "void tmem_ld_wait(uint32_t (&r)[N])" in src
+    lines = src.split("\n")
+    for i, line in enumerate(lines):
+        for words in re.findall(r"tmem_ld(?:16|32)\(t_addr[^;]*, (\w+)\);", line):
+            assert any(f"tmem_ld_wait({words})" in x for x in lines[i:i + 16]), line
+    assert not re.search(r"tmem_ld_wait\(\s*\)", src)
