@@ -264,10 +264,34 @@ __device__ __forceinline__ void fill_x(const XT* x, int64_t k, int m, int chunks
   if (total == 0) meanwhile();
 }
 
+// The sum of an element of y by the formula as it stands, over k = first, first + step, ...
+template <typename XT>
+__device__ __forceinline__ float w4_dot(const W4Args& a, int i, int n, int first, int step) {
+  const uint8_t* q = a.q + (int64_t)n * (a.k >> 1);
+  const XT* x = static_cast<const XT*>(a.x) + (int64_t)i * a.k;
+  const int groups = a.k / a.group;
+  float sum = 0.f;
+  for (int k = first; k < a.k; k += step) {
+    const int64_t o = (int64_t)n * groups + k / a.group;
+    const int code = (q[k >> 1] >> (4 * (k & 1))) & 15;
+    const float z = a.zero != nullptr ? (float)a.zero[o] : 8.f;
+    const float w = __half2float(a.w_scale[o]) * ((float)code - z);
+    sum = fmaf(w, (float)x[k], sum);
+  }
+  return sum;
+}
+// An element whose sum on the tensor cores is not finite.  There an infinite x meets -z sum x and the code apart, and makes a
+// NaN of what may be an infinity (so does an infinite scale): one thread takes the sum again.
+__device__ __noinline__ float w4_sum_again(const W4Args& a, int x_dtype, int i, int n) {
+  if (x_dtype == DTAS_F16) return w4_dot<__half>(a, i, n, 0, 1);
+  if (x_dtype == DTAS_I8) return w4_dot<int8_t>(a, i, n, 0, 1);
+  return w4_dot<__nv_fp8_e4m3>(a, i, n, 0, 1);
+}
+
 // GS steps share a scale: 1, 2, or 4 (groups of 128 and more).
 template <int IK, int NT, int GS, bool ZERO>
 __global__ void __launch_bounds__(kThreads, 1)
-    gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const W4Args a, const W4Shape sh) {
+    gemv_w4_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ W4Args a, const W4Shape sh) {
   using It = Item<IK, GS, ZERO>;
   extern __shared__ uint8_t w4_smem_raw[];
   // With groups of 128 k and more, lane t takes the codes 32 t .. 32 t + 31 of 128 (one 16-byte read a row), a word of
@@ -413,6 +437,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto finish = [&](int i, int col, float4 sum) {
     float v[4] = {sum.x, sum.y, sum.z, sum.w};
     const float unit = a.x_scale != nullptr ? 0x1p24f * a.x_scale[i] : 0x1p24f;
+    if (!(fabsf(v[0]) + fabsf(v[1]) + fabsf(v[2]) + fabsf(v[3]) < INFINITY)) {
+#pragma unroll 1
+      for (int e = 0; e < 4; ++e)
+        if (col + e < a.n && !(fabsf(v[e]) < INFINITY)) v[e] = w4_sum_again(a, sh.x_dtype, i, col + e) * 0x1p-24f;
+    }
     if (col + 4 <= a.n && !a.epi.out_f32 && (reinterpret_cast<uintptr_t>(a.y) & 7) == 0 && (a.n & 3) == 0) {
       __half h[4];
 #pragma unroll
@@ -674,17 +703,7 @@ __global__ void __launch_bounds__(256) gemv_w4_scalar_kernel(const W4Args a) {
   pdl_wait();
   pdl_launch_dependents();
   if (n >= a.n) return;
-  const uint8_t* q = a.q + (int64_t)n * (a.k >> 1);
-  const XT* x = static_cast<const XT*>(a.x) + (int64_t)i * a.k;
-  const int groups = a.k / a.group;
-  float sum = 0.f;
-  for (int k = lane; k < a.k; k += 32) {
-    const int gi = k / a.group;
-    const int code = (q[k >> 1] >> (4 * (k & 1))) & 15;
-    const float z = a.zero != nullptr ? (float)a.zero[(int64_t)n * groups + gi] : 8.f;
-    const float w = __half2float(a.w_scale[(int64_t)n * groups + gi]) * ((float)code - z);
-    sum = fmaf(w, (float)x[k], sum);
-  }
+  float sum = w4_dot<XT>(a, i, n, lane, 32);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) {

@@ -1,9 +1,11 @@
 """The low-bit path on the GPU where a result is known exactly, and at its edges: values halfway between two 8-bit ones, residuals
-of other shapes and strides."""
+of other shapes and strides, infinities."""
+import math
+
 import pytest
 import torch
 
-from dtas_b200 import _abi, ops
+from dtas_b200 import _abi, ops, weights
 
 pytestmark = pytest.mark.gpu
 
@@ -99,3 +101,44 @@ def test_residuals_of_other_shapes_are_refused(cuda_device):
                 with pytest.raises(_abi.DtasError):
                     call()
     assert (out == 3.0).all()
+
+
+# ---- 4-bit products: what is not finite --------------------------------------------------------------
+def w4_operands(m, n, k, group, zero, seed=0):
+    """x, codes [N, K], packed codes, scales, zero points or None."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    codes = torch.randint(0, 16, (n, k), generator=g, device="cuda", dtype=torch.uint8)
+    scales = (0.01 + 0.01 * torch.rand(n, k // group, generator=g, device="cuda")).to(F16)
+    zeros = torch.randint(0, 16, (n, k // group), generator=g, device="cuda", dtype=torch.uint8) if zero else None
+    return torch.randn(m, k, generator=g, device="cuda").to(F16), codes, weights.pack_w4(codes), scales, zeros
+
+
+def w4_matrix(codes, scales, zeros):
+    n, groups = scales.shape
+    z = 8.0 if zeros is None else zeros.double()[..., None]
+    return ((codes.double().view(n, groups, -1) - z) * scales.double()[..., None]).view(n, -1)
+
+
+@pytest.mark.parametrize("zero", [False, True])
+@pytest.mark.parametrize("m,n,k,group", [(4, 70, 128, 64), (4, 70, 60, 30), (1, 33, 4096, 128), (7, 100, 1056, 32), (16, 200, 11008, 128)])
+def test_gemv_w4_infinities_are_those_of_the_formula(cuda_device, m, n, k, group, zero):
+    """An infinite x gives an infinity by the sign of code - zero, a NaN where that is 0; two of them, or a NaN, what their sum is.
+    The same from both kernels, and nothing in the other rows."""
+    x, codes, packed, scales, zeros = w4_operands(m, n, k, group, zero, seed=k)
+    x[0, k // 3] = math.inf
+    if m > 2:
+        x[1, k - 1], x[1, 2] = -math.inf, math.inf
+        x[2, 5] = math.nan
+    scales[5, 0] = math.inf
+    w = w4_matrix(codes, scales, zeros)
+    out = torch.empty(m, n, dtype=F16, device="cuda")
+    ops.gemv_w4(x, packed, scales, out, w_zero=zeros)
+    # the products one by one: a matrix product may take infinities in any order, but no order changes these
+    for i in range(m):
+        want = (x[i].double() * w).sum(-1)
+        assert torch.equal(torch.isnan(out[i]), torch.isnan(want)), i
+        assert torch.equal(torch.isinf(out[i]), torch.isinf(want)), i
+        inf = torch.isinf(want)
+        assert torch.equal(out[i][inf].double(), want[inf])
+        if i not in (0, 1, 2):
+            assert torch.isfinite(out[i][torch.arange(n, device="cuda") != 5].float()).all()
