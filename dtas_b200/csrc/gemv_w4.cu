@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int quad = (lane & 7) * 4, row4 = lane >> 3;
   auto finish = [&](int i, int col, float4 sum) {
     float v[4] = {sum.x, sum.y, sum.z, sum.w};
-    const float unit = a.x_scale != nullptr ? 0x1p24f * a.x_scale[i] : 0x1p24f;
+    const float scale = a.x_scale != nullptr ? a.x_scale[i] : 1.f;
     if (!(fabsf(v[0]) + fabsf(v[1]) + fabsf(v[2]) + fabsf(v[3]) < INFINITY)) {
 #pragma unroll 1
       for (int e = 0; e < 4; ++e)
@@ -445,12 +445,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (col + 4 <= a.n && !a.epi.out_f32 && (reinterpret_cast<uintptr_t>(a.y) & 7) == 0 && (a.n & 3) == 0) {
       __half h[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) h[e] = __float2half_rn(epi_value(a.epi, v[e] * unit, i, col + e));
+      for (int e = 0; e < 4; ++e) h[e] = __float2half_rn(epi_value(a.epi, v[e] * 0x1p24f * scale, i, col + e));
       *reinterpret_cast<uint2*>(static_cast<__half*>(a.y) + (int64_t)i * a.n + col) = *reinterpret_cast<const uint2*>(h);
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (col + e < a.n) epi_store(a.epi, a.y, a.n, i, col + e, epi_value(a.epi, v[e] * unit, i, col + e));
+        if (col + e < a.n) epi_store(a.epi, a.y, a.n, i, col + e, epi_value(a.epi, v[e] * 0x1p24f * scale, i, col + e));
     }
   };
   // This CTA's sums of tile `tl` of a batch for row i of x: the result, or what the CTA that finishes the row is sent.

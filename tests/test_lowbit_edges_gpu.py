@@ -142,3 +142,85 @@ def test_gemv_w4_infinities_are_those_of_the_formula(cuda_device, m, n, k, group
         assert torch.equal(out[i][inf].double(), want[inf])
         if i not in (0, 1, 2):
             assert torch.isfinite(out[i][torch.arange(n, device="cuda") != 5].float()).all()
+
+
+@pytest.mark.parametrize("k", [128, 60])
+def test_gemv_w4_with_row_scales_at_the_ends_of_fp32(cuda_device, k):
+    """Rows of 8 bits whose scale is very large or very small, as those of fp32 rows may be: their sums times the scale, 0 where the sum
+    is 0."""
+    n, group = 40, k // 2
+    _, codes, packed, _, _ = w4_operands(1, n, k, group, False, seed=1)
+    codes[7] = 8                                           # a row of zeros: its sums are 0 whatever the scale
+    packed = weights.pack_w4(codes)
+    scales = torch.full((n, 2), 2.0 ** -14, dtype=F16, device="cuda")
+    x = torch.ones(4, k, dtype=I8, device="cuda")
+    x_scale = torch.tensor([2.0 ** 127, 2.0 ** 104, 2.0 ** -140, 1.0], device="cuda")
+    out = torch.empty(4, n, dtype=F32, device="cuda")
+    ops.gemv_w4(x, packed, scales, out, x_scale=x_scale)
+    want = ((codes.double() - 8).sum(-1) * 2.0 ** -14 * x_scale.double()[:, None]).to(F16).float()
+    assert torch.equal(out, want)
+
+
+# ---- stream order ------------------------------------------------------------------------------------
+class Chain:
+    """Every operand of a low-bit call - activations, scales, weights, biases - is written by the call right before
+    it, buffers are reused, and nothing synchronises in between: kernels start while the one before them still runs."""
+
+    def __init__(self, m, h, f):
+        g = torch.Generator(device="cuda").manual_seed(5)
+        rand = lambda *shape, s=1.0: (torch.randn(*shape, generator=g, device="cuda") * s).to(F16)  # noqa: E731
+        new = lambda *shape, dt=F16: torch.zeros(*shape, dtype=dt, device="cuda")  # noqa: E731
+        self.m = m
+        self.norms, self.biases = [rand(1, h) for _ in range(2)], [rand(1, f, s=0.1) for _ in range(2)]
+        self.downs = [rand(h, f, s=0.05) for _ in range(2)]
+        self.ups = [weights.quantize_w4(rand(f, h, s=0.05), 32, True) for _ in range(2)]
+        self.x0, self.res0 = rand(m, h), rand(m, h)
+        self.x, self.res, self.norm, self.bias = new(m, h), new(m, h), new(1, h), new(1, f)
+        self.codes, self.scales, self.zeros = (torch.zeros_like(t) for t in self.ups[0])
+        self.h8, self.hs, self.u = new(m, h, dt=E4M3), new(m, dt=F32), new(m, f)
+        self.u8, self.us, self.w8, self.ws, self.y = new(m, f, dt=E4M3), new(m, dt=F32), new(h, f, dt=E4M3), new(h, dt=F32), new(m, h)
+        self.outs = [new(m, h) for _ in range(4)]
+
+    def run(self, sync):
+        def call(op, *args, **kw):
+            op(*args, **kw)
+            if sync:
+                torch.cuda.synchronize()
+
+        call(ops.copy, self.x0, self.x)
+        call(ops.copy, self.res0, self.res)
+        for i in range(4):
+            up = self.ups[i % 2]
+            call(ops.copy, self.norms[i % 2], self.norm)
+            call(ops.add_rms_norm, self.x, self.res, self.norm, self.h8, res_out=self.res, scale=self.hs)
+            call(ops.copy, up[2].view(I8), self.zeros.view(I8))
+            call(ops.copy, up[1], self.scales)
+            call(ops.copy, up[0].view(I8), self.codes.view(I8))
+            call(ops.copy, self.biases[i % 2], self.bias)
+            call(ops.gemv_w4, self.h8, self.codes, self.scales, self.u, w_zero=self.zeros, x_scale=self.hs, bias=self.bias, act="gelu")
+            call(ops.gemv_w4, self.res, self.codes, self.scales, self.u, w_zero=self.zeros, res1=self.u)
+            call(ops.quantize, self.downs[i % 2], self.w8, self.ws)
+            call(ops.quantize, self.u, self.u8, self.us)
+            call(ops.gemm_nt_f8, self.u8, self.w8, self.us, self.ws, self.y, res1=self.res)
+            call(ops.add_rms_norm, self.y, None, self.norm, self.x)
+            call(ops.copy, self.x, self.outs[i])
+        return [o.clone() for o in self.outs]
+
+
+@pytest.mark.parametrize("m,h,f", [(1, 1024, 4096), (16, 2560, 2816), (5, 1025 * 32, 96), (3, 4096, 11008)])
+def test_calls_keep_stream_order(cuda_device, m, h, f):
+    chain = Chain(m, h, f)
+    want = chain.run(sync=True)
+    assert all(torch.isfinite(o.float()).all() for o in want) and not torch.equal(want[0], want[1])
+    for _ in range(20):
+        assert all(torch.equal(a, b) for a, b in zip(chain.run(sync=False), want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        chain.run(sync=False)
+    for _ in range(20):
+        for o in chain.outs:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(chain.outs, want))
+    ops.poll_status()
