@@ -54,13 +54,14 @@ __device__ __forceinline__ void mma_16816(float* c, const uint32_t* a, uint32_t 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Eight consecutive elements of a row of x, as loaded, and as pairs (k, k + 4) of fp16 numbers.
+// Eight consecutive elements of a row of x, as loaded, and as pairs (k, k + 4) of fp16 numbers.  Ordinary loads, not those
+// of the read-only path: the kernel before this one may be writing x still when this one begins (pdl_wait).
 template <typename XT>
 struct XVec;
 template <>
 struct XVec<__half> {
   uint4 r;
-  __device__ __forceinline__ void load(const __half* p) { r = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void load(const __half* p) { r = *reinterpret_cast<const uint4*>(p); }
   __device__ __forceinline__ void pairs(uint32_t* p) const {      // (0, 4), (1, 5), (2, 6), (3, 7)
     p[0] = __byte_perm(r.x, r.z, 0x5410);
     p[1] = __byte_perm(r.x, r.z, 0x7632);
@@ -71,7 +72,7 @@ struct XVec<__half> {
 template <>
 struct XVec<int8_t> {
   uint2 r;
-  __device__ __forceinline__ void load(const int8_t* p) { r = __ldg(reinterpret_cast<const uint2*>(p)); }
+  __device__ __forceinline__ void load(const int8_t* p) { r = *reinterpret_cast<const uint2*>(p); }
   __device__ __forceinline__ void pairs(uint32_t* p) const {
     const uint32_t a = r.x ^ 0x80808080u, b = r.y ^ 0x80808080u;      // x + 128 in 0..255
     const __half2 bias = __float2half2_rn(1152.f);                    // 1024 + 128
@@ -86,7 +87,7 @@ struct XVec<int8_t> {
 template <>
 struct XVec<__nv_fp8_e4m3> {
   uint2 r;
-  __device__ __forceinline__ void load(const __nv_fp8_e4m3* p) { r = __ldg(reinterpret_cast<const uint2*>(p)); }
+  __device__ __forceinline__ void load(const __nv_fp8_e4m3* p) { r = *reinterpret_cast<const uint2*>(p); }
   __device__ __forceinline__ void pairs(uint32_t* p) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

@@ -67,3 +67,10 @@ def test_every_wait_for_tensor_memory_names_its_registers():
         for words in re.findall(r"tmem_ld(?:16|32)\(t_addr[^;]*, (\w+)\);", line):
             assert any(f"tmem_ld_wait({words})" in x for x in lines[i:i + 16]), line
     assert not re.search(r"tmem_ld_wait\(\s*\)", src)
+
+
+def test_activations_do_not_take_the_read_only_path():
+    """A kernel may begin while the one that writes its x still runs: loads that promise that x does not change while
+    the kernel runs (ld.global.nc) are not for it."""
+    src = open(os.path.join(CSRC, "gemv_w4.cu")).read()
+    assert "__ldg" not in src and "ld.global.nc" not in src
