@@ -265,28 +265,47 @@ __device__ __forceinline__ void fill_x(const XT* x, int64_t k, int m, int chunks
   if (total == 0) meanwhile();
 }
 
-// The sum of an element of y by the formula as it stands, over k = first, first + step, ...
+// An element of y whose sum on the tensor cores, v, is not finite.  There an infinite x meets -z sum x and the code
+// apart, which makes a NaN of what may be an infinity (so does an infinite scale).  Beside such terms the finite ones do not
+// matter: one thread looks for them - at k whose x, and in groups whose scale is not finite - and adds up those alone,
+// until they make a NaN.
 template <typename XT>
-__device__ __forceinline__ float w4_dot(const W4Args& a, int i, int n, int first, int step) {
-  const uint8_t* q = a.q + (int64_t)n * (a.k >> 1);
+__device__ __forceinline__ float w4_not_finite(const W4Args& a, int i, int n, float v) {
   const XT* x = static_cast<const XT*>(a.x) + (int64_t)i * a.k;
   const int groups = a.k / a.group;
+  const __half* scales = a.w_scale + (int64_t)n * groups;
   float sum = 0.f;
-  for (int k = first; k < a.k; k += step) {
-    const int64_t o = (int64_t)n * groups + k / a.group;
-    const int code = (q[k >> 1] >> (4 * (k & 1))) & 15;
-    const float z = a.zero != nullptr ? (float)a.zero[o] : 8.f;
-    const float w = __half2float(a.w_scale[o]) * ((float)code - z);
-    sum = fmaf(w, (float)x[k], sum);
+  bool found = false;
+  auto add = [&](int k) {
+    const int code = (a.q[(int64_t)n * (a.k >> 1) + (k >> 1)] >> (4 * (k & 1))) & 15;
+    const float z = a.zero != nullptr ? (float)a.zero[(int64_t)n * groups + k / a.group] : 8.f;
+    sum = fmaf(__half2float(scales[k / a.group]) * ((float)code - z), (float)x[k], sum);
+    found = true;
+  };
+#pragma unroll 1
+  for (int k = 0; k < a.k && sum == sum; k += 8) {
+    XVec<XT> c;
+    uint32_t p[4];
+    c.load(x + k);
+    c.pairs(p);
+    bool any = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) any = any || (p[j] & 0x7c00u) == 0x7c00u || (p[j] & 0x7c000000u) == 0x7c000000u;
+    if (any)
+#pragma unroll 1
+      for (int j = k; j < k + 8; ++j)
+        if (!(fabsf((float)x[j]) < INFINITY)) add(j);
   }
-  return sum;
+#pragma unroll 1
+  for (int gi = 0; gi < groups && sum == sum; ++gi)
+    if (!(fabsf(__half2float(scales[gi])) < INFINITY))
+      for (int k = gi * a.group; k < (gi + 1) * a.group; ++k) add(k);
+  return found ? sum * 0x1p-24f : v;
 }
-// An element whose sum on the tensor cores is not finite.  There an infinite x meets -z sum x and the code apart, and makes a
-// NaN of what may be an infinity (so does an infinite scale): one thread takes the sum again.
-__device__ __noinline__ float w4_sum_again(const W4Args& a, int x_dtype, int i, int n) {
-  if (x_dtype == DTAS_F16) return w4_dot<__half>(a, i, n, 0, 1);
-  if (x_dtype == DTAS_I8) return w4_dot<int8_t>(a, i, n, 0, 1);
-  return w4_dot<__nv_fp8_e4m3>(a, i, n, 0, 1);
+__device__ __noinline__ float w4_not_finite(const W4Args& a, int x_dtype, int i, int n, float v) {
+  if (x_dtype == DTAS_F16) return w4_not_finite<__half>(a, i, n, v);
+  if (x_dtype == DTAS_I8) return w4_not_finite<int8_t>(a, i, n, v);
+  return w4_not_finite<__nv_fp8_e4m3>(a, i, n, v);
 }
 
 // GS steps share a scale: 1, 2, or 4 (groups of 128 and more).
@@ -437,12 +456,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int quad = (lane & 7) * 4, row4 = lane >> 3;
   auto finish = [&](int i, int col, float4 sum) {
     float v[4] = {sum.x, sum.y, sum.z, sum.w};
-    const float scale = a.x_scale != nullptr ? a.x_scale[i] : 1.f;
     if (!(fabsf(v[0]) + fabsf(v[1]) + fabsf(v[2]) + fabsf(v[3]) < INFINITY)) {
 #pragma unroll 1
       for (int e = 0; e < 4; ++e)
-        if (col + e < a.n && !(fabsf(v[e]) < INFINITY)) v[e] = w4_sum_again(a, sh.x_dtype, i, col + e) * 0x1p-24f;
+        if (col + e < a.n && !(fabsf(v[e]) < INFINITY)) v[e] = w4_not_finite(a, sh.x_dtype, i, col + e, v[e]);
     }
+    const float scale = a.x_scale != nullptr ? a.x_scale[i] : 1.f;
     if (col + 4 <= a.n && !a.epi.out_f32 && (reinterpret_cast<uintptr_t>(a.y) & 7) == 0 && (a.n & 3) == 0) {
       __half h[4];
 #pragma unroll
@@ -704,7 +723,17 @@ __global__ void __launch_bounds__(256) gemv_w4_scalar_kernel(const W4Args a) {
   pdl_wait();
   pdl_launch_dependents();
   if (n >= a.n) return;
-  float sum = w4_dot<XT>(a, i, n, lane, 32);
+  const uint8_t* q = a.q + (int64_t)n * (a.k >> 1);
+  const XT* x = static_cast<const XT*>(a.x) + (int64_t)i * a.k;
+  const int groups = a.k / a.group;
+  float sum = 0.f;
+  for (int k = lane; k < a.k; k += 32) {
+    const int gi = k / a.group;
+    const int code = (q[k >> 1] >> (4 * (k & 1))) & 15;
+    const float z = a.zero != nullptr ? (float)a.zero[(int64_t)n * groups + gi] : 8.f;
+    const float w = __half2float(a.w_scale[(int64_t)n * groups + gi]) * ((float)code - z);
+    sum = fmaf(w, (float)x[k], sum);
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) {
