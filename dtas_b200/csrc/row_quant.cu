@@ -610,12 +610,15 @@ inline RowPlan row_plan(int64_t m, int64_t n_cols, bool aligned, bool norm, bool
 
 template <int OP, typename InT, typename OutT, int CH, bool EDGE>
 int launch_stream(const RowPlan& p, const RowArgs& a, int sm_count, cudaStream_t st) {
-  static std::atomic<int> per_sm[kMaxThreads / 32 + 1];      // CTAs of so many warps that an SM holds, once asked for
+  static std::atomic<int> per_sm[64][kMaxThreads / 32 + 1];      // [device]: CTAs of so many warps that an SM holds, once asked for
   const int threads = p.tpr * p.rows;
-  int fit = per_sm[threads / 32].load(std::memory_order_relaxed);
+  int dev = 0;
+  DTAS_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64) DTAS_FAIL(DTAS_EINVAL, "row op: device ordinal %d out of range", dev);
+  int fit = per_sm[dev][threads / 32].load(std::memory_order_relaxed);
   if (fit == 0) {
     DTAS_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, (row_quant_stream_kernel<OP, InT, OutT, CH, EDGE>), threads, 0));
-    per_sm[threads / 32].store(fit, std::memory_order_relaxed);
+    per_sm[dev][threads / 32].store(fit, std::memory_order_relaxed);
   }
   const int64_t groups = (a.m + p.rows - 1) / p.rows, most = (int64_t)sm_count * fit;
   launch_kernel((row_quant_stream_kernel<OP, InT, OutT, CH, EDGE>), (unsigned)(groups < most ? groups : most), dim3(p.tpr, p.rows), 0,
