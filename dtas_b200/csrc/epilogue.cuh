@@ -44,9 +44,9 @@ struct PeerOut {
   void* mc = nullptr;
 };
 
-// Host and device: true when finishing an element costs more than a bias add and a store.
+// Host and device: true when finishing an element of fp16 operands costs more than a bias add and a store.
 inline __host__ __device__ bool epi_has_work(const Epilogue& e) {
-  return e.act != DTAS_ACT_NONE || e.res1 != nullptr || e.sx != nullptr;
+  return e.act != DTAS_ACT_NONE || e.res1 != nullptr;
 }
 
 #ifdef __CUDACC__

@@ -1278,36 +1278,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairMaxThreads, 1)
       const int mt = sg.mt, nt = sg.nt;
       const int acc = iter & 1;
       const uint32_t acc_phase = (uint32_t)(iter >> 1) & 1u;
-      float row_scale = 0.f, my_scale[2] = {0.f, 0.f};
-      __half my_bias[2] = {__half(0.f), __half(0.f)};
+      float row_scale = 0.f, my_scale = 0.f;
+      __half my_bias = __half(0.f);
       if constexpr (F8) {
         // The main loop of an e4m3 tile is half as long as an fp16 tile's, too short to hide a trip to L2 for every 32
         // columns' scales and bias behind it (1000 x 10240 x 2560 with bias: 39.5 us so, 30.5 this way, 27.3 without
-        // bias): a thread fetches its columns' (one of eight warps, two of four) while the tile is computed, and they
-        // wait in shared memory for the arithmetic.
+        // bias): each of the 256 epilogue threads fetches its column's while the tile is computed, and they wait in
+        // shared memory for the arithmetic.
         const int r = mt * 2 * BM + (int)rank * BM + quarter * 32 + lane;
         if (r < a.m) row_scale = a.epi.sx[r];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int c = epi_tid + e * n_epi_threads, col = nt * kPairBN + c;
-          if (c < kPairBN && col < a.n) {
-            my_scale[e] = a.epi.sw[col];
-            if (a.epi.bias != nullptr) my_bias[e] = a.epi.bias[col];
-          }
+        const int col = nt * kPairBN + epi_tid;
+        if (col < a.n) {
+          my_scale = a.epi.sw[col];
+          if (a.epi.bias != nullptr) my_bias = a.epi.bias[col];
         }
       }
       ok = mbar_wait(tfull_bar(acc), acc_phase, a.status, ERR_EPILOGUE);
       if constexpr (F8) {
         ok = epilogue_bar_and_n(n_epi_threads, ok);      // all go on or all leave; the tile before is done with its columns
         if (!ok) break;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int c = epi_tid + e * n_epi_threads;
-          if (c < kPairBN) {
-            col_scale[c] = my_scale[e];
-            col_bias[c] = my_bias[e];
-          }
-        }
+        col_scale[epi_tid] = my_scale;
+        col_bias[epi_tid] = my_bias;
         epilogue_bar_sync_n(n_epi_threads);
       }
       if (!ok) break;
@@ -1505,7 +1496,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairMaxThreads, 1)
         // bytes), a block ahead, and are laid out in the stage, where the results then take their places.  Ragged and
         // unaligned ones are read in place.
         const bool by_rows = DTAS_PAIR_STAGED_STORE && a.epi.vec_res && a.vec_store && !a.epi.out_f32 &&
-                             col_base + c_end * 32 <= a.n && (c_end & 1) == 0;
+                             col_base + c_end * 32 <= a.n;
         const int row0 = mt * 2 * BM + (int)rank * BM + quarter * 32;
         uint4 ahead[8];
         auto fetch = [&](int c) {
@@ -2454,7 +2445,8 @@ int launch_pair(const CUtensorMap& tx, const CUtensorMap& tw, const GemmArgs& a,
   }
   // twice the epilogue warps when there is an activation or a residual to work through per element, or
   // partial tiles to read back (the read rate of a CTA grows with the warps that issue the loads)
-  const int threads = (epi_has_work(a.epi) || ap.sk_per > 0) ? kPairMaxThreads : kGemmThreads;
+  static_assert(kPairMaxThreads - 64 == kPairBN, "e4m3: an epilogue thread per column of a tile");
+  const int threads = (F8 || epi_has_work(a.epi) || ap.sk_per > 0) ? kPairMaxThreads : kGemmThreads;
   launch_kernel(gemm_f16_tcgen05_pair_kernel<F8, RES>, 2 * pairs, threads, kSmem, st, tx, tw, ap);
   return after_launch("gemm_f16_tcgen05_pair_kernel");
 }

@@ -682,9 +682,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (n_items > 0) {
         const int u0 = tl * n_items, w0 = u0 / per, w1 = (u0 + n_items - 1) / per;
         if (w0 == w1) continue;             // that warp has done it
-        if (i < a.m) {                      // area 1 of the first, unless its run begins inside the tile; area 0 of the others
+        if (i < a.m) {                      // area 1 of the warp whose run holds the tile's first item; area 0 of the others
           const float* from = part + i * kRows + quad;
-          add4(sum, from + (2 * w0 + (w0 * per > u0 ? 0 : 1)) * (a.m * kRows));
+          add4(sum, from + (2 * w0 + 1) * (a.m * kRows));
           for (int w = w0 + 1; w <= w1; ++w) add4(sum, from + 2 * w * (a.m * kRows));
         }
       }
