@@ -1,11 +1,17 @@
-"""The low-bit path on the GPU where a result is known exactly, and at its edges: values halfway between two 8-bit ones, residuals
-of other shapes and strides, infinities."""
+"""The low-bit path on the GPU where a result is known exactly, and at its edges: values halfway between two 8-bit ones, products of
+small whole numbers, residuals of other shapes and strides, infinities, odd addresses, stream order.
+
+The products' operands are whole numbers and powers of two wherever a result is compared for equality: every partial sum is then a
+whole number below 2^24 (times a power of two) and exact in fp32 whatever its order, so the one rounding to fp16 is all there
+is, and a k that is lost, taken twice or scaled by another group's scale shows."""
 import math
 
 import pytest
 import torch
 
 from dtas_b200 import _abi, ops, weights
+
+from tests.test_lowbit_gpu import CODES, SMALL_CODES, assert_fp16_close, gelu, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -85,6 +91,139 @@ def test_rows_of_fp16_numbers_are_rounded_once(cuda_device, dtype):
     ops.quantize(x, q, scale)
     y = x.double() * Q[dtype] / x.double().abs().amax(-1, keepdim=True)
     assert torch.equal(q.float(), (y.round() if dtype == I8 else y.to(F32).to(E4M3)).float())
+
+
+@pytest.mark.parametrize("h", [600, 1030, 4100, 8000, 8720, 17408, 20000])
+def test_rows_at_odd_addresses_are_the_same_rows(cuda_device, h):
+    """Neither a maximum nor a product depends on how a row is cut: the 8-bit rows are those of the aligned call."""
+    m = 5
+    for in_dtype in (F16, F32):
+        x, res, weight = randn(m, h, seed=1).to(in_dtype), randn(m, h, seed=2).to(in_dtype), (1 + randn(h, seed=3, scale=0.1)).to(F16)
+        buf = torch.zeros(m * h + 8, dtype=in_dtype, device="cuda")
+        odd = buf[3:3 + m * h].view(m, h)
+        odd.copy_(x)
+        for dtype in (I8, E4M3):
+            rows, scales, sums = [], [], []
+            for a in (x, odd):
+                out = torch.zeros(m * h + 8, dtype=torch.uint8, device="cuda")
+                q = out[a is odd:][:m * h].view(dtype).view(m, h)
+                scale, total = torch.empty(m, device="cuda"), torch.empty_like(x)
+                ops.quantize(a, q, scale)
+                rows.append(q.float()), scales.append(scale)
+                q, s = torch.empty(m, h, dtype=dtype, device="cuda"), torch.empty(m, device="cuda")
+                ops.add_rms_norm(a, res, weight, q, res_out=total, scale=s)
+                rows.append(q.float()), scales.append(s), sums.append(total)
+                assert (out[m * h + (a is odd):] == 0).all()
+            assert torch.equal(rows[0], rows[2]) and torch.equal(rows[1], rows[3]) and torch.equal(sums[0], sums[1])
+            assert torch.equal(scales[0], scales[2])
+            assert ((scales[1] - scales[3]).abs() <= scales[1] * 2.0 ** -18).all()      # another order of the sum of squares
+
+
+# ---- products of whole numbers -----------------------------------------------------------------------
+def whole(*shape, top, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randint(-top, top + 1, shape, generator=g, device="cuda")
+
+
+def power(*shape, lo, hi, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return 2.0 ** torch.randint(lo, hi + 1, shape, generator=g, device="cuda").double()
+
+
+W4_SHAPES = [(1, 32, 32), (70, 32, 32), (33, 1056, 32), (40, 64, 64), (31, 192, 64), (100, 4096, 128), (64, 4064, 32), (4099, 256, 32), (50, 11008, 128),
+             (300, 20480, 64), (40, 768, 384), (70, 1536, 512), (35, 640, 640), (260, 2560, 64), (17, 60, 30), (9, 6, 3), (12, 2, 1)]
+
+
+@pytest.mark.parametrize("zero", [False, True])
+@pytest.mark.parametrize("x_dtype", [F16, I8, E4M3])
+@pytest.mark.parametrize("n,k,group", W4_SHAPES)
+def test_gemv_w4_of_whole_numbers(cuda_device, n, k, group, x_dtype, zero):
+    for m in (1, 3, 8, 9, 16):
+        x = whole(m, k, top=2, seed=m)
+        codes = whole(n, k, top=7, seed=k) + 7 + (whole(n, k, top=1, seed=k + 1) > 0)       # 0 .. 15
+        scales = power(n, k // group, lo=-2, hi=1, seed=n)
+        zeros = (whole(n, k // group, top=7, seed=5) + 8).to(torch.uint8) if zero else None   # 1 .. 15
+        x_scale = None if x_dtype == F16 else power(m, lo=-3, hi=3, seed=6).float()
+        w = w4_matrix(codes, scales, zeros)
+        want = (x.double() @ w.t()) * (1.0 if x_scale is None else x_scale.double()[:, None])
+        bias, r1, r2 = (whole(*s, top=64, seed=7).to(F16) for s in ((n,), (m, n), (m, n)))
+        # a row's sums: at most 2 * 15 * 20480 times a scale of 2, in steps of 2^-2, so below 2^23 steps; the row's scale moves
+        # the exponent alone, and bias and residuals, up to 192 in steps of 1, add less than 2^13 steps of 2^-5
+        for kw, add in (({}, 0), ({"bias": bias}, bias.double()), ({"res1": r1, "res2": r2}, r1.double() + r2.double())):
+            out = torch.empty(m, n, dtype=F16, device="cuda")
+            ops.gemv_w4(x.to(x_dtype if x_dtype != E4M3 else F32).to(x_dtype), weights.pack_w4(codes.to(torch.uint8)), scales.to(F16), out,
+                        w_zero=zeros, x_scale=x_scale, **kw)
+            assert torch.equal(out.float(), (want + add).to(F32).to(F16).float()), (m, list(kw))
+
+
+@pytest.mark.parametrize("x_dtype", [F16, I8])
+@pytest.mark.parametrize("m,n,k,group", [(1, 300, 4096, 128), (5, 300, 4096, 32), (16, 300, 11008, 128), (9, 200, 20480, 64), (2, 100, 4064, 32)])
+def test_gemv_w4_roundings(cuda_device, m, n, k, group, x_dtype):
+    """Accumulators of the MMAs restart with every group, or every 128 k of a longer one, so they see at most four steps, of two
+    truncations to 2^-23 each, of sums bounded by the codes' (30 s |x|, as zero points enter apart); the sums of x
+    a dozen roundings of 2^-24.  Two fused multiply-adds per group in a row's fp32 sum, and the joins of at most 12 warps and 8 CTAs,
+    are roundings of 2^-24 of a sum bounded by |x| |w|."""
+    _, codes, packed, scales, zeros = w4_operands(m, n, k, group, True, seed=k)
+    x = randn(m, k, seed=m)
+    x_scale = None
+    if x_dtype == I8:
+        x_scale, x = torch.full((m,), 0.03, device="cuda"), (x * 30).round().clamp(-127, 127)
+    w = w4_matrix(codes, scales, zeros)
+    out = torch.empty(m, n, dtype=F16, device="cuda")
+    ops.gemv_w4(x.to(x_dtype), packed, scales, out, w_zero=zeros, x_scale=x_scale)
+    xd = x.to(x_dtype).double() * (1.0 if x_scale is None else x_scale.double()[:, None])
+    codes_mag = xd.abs() @ (30 * scales.double()).repeat_interleave(group, 1).t()
+    sum_mag = xd.abs() @ w.abs().t()
+    assert_fp16_close(out, xd @ w.t(), codes_mag * ((8 + 6) * 2.0 ** -23) + sum_mag * ((2 * k // min(group, 128) + 24) * 2.0 ** -24))
+
+
+@pytest.fixture
+def in_kernel():
+    lib = _abi.lib()
+    yield lambda code: _abi.check(lib.dtas_gemm_set_override(*code))
+    lib.dtas_gemm_set_override(0, 0)
+
+
+@pytest.mark.parametrize("n", [328, 333, 512])
+@pytest.mark.parametrize("m,code", [(m, c) for m in (200, 333) for c in CODES] + [(m, c) for m in (1, 20, 50) for c in SMALL_CODES] + [(513, (0, 0)), (2, (0, 0))])
+def test_gemm_f8_of_whole_numbers_in_every_kernel(cuda_device, in_kernel, m, code, n):
+    """Residuals as views of wider buffers, one and two of them, ragged and whole tiles; results as they are, as fp32 and in a slab."""
+    k = 1616
+    x, w = whole(m, k, top=2, seed=m), whole(n, k, top=2, seed=n)
+    sx, sw = power(m, lo=-3, hi=3, seed=1), power(n, lo=-3, hi=3, seed=2)
+    y = (x.double() @ w.double().t()) * sx[:, None] * sw
+    bias = whole(n, top=64, seed=3).to(F16)
+    wide = whole(2, m, n + 24, top=64, seed=4).to(F16)
+    r1, r2 = wide[0][:, 8:8 + n], wide[1][:, 16:16 + n]
+    x8, w8 = x.float().to(E4M3), w.float().to(E4M3)
+    in_kernel(code)
+    for kw, add in (({}, 0), ({"bias": bias}, bias.double()), ({"res1": r1}, r1.double()), ({"bias": bias, "res1": r1, "res2": r2}, bias.double() + r1.double() + r2.double()),
+                    ({"res1": r1.contiguous(), "res2": r2.contiguous()}, r1.double() + r2.double())):
+        want = (y + add).to(F32).to(F16)
+        for dtype in (F16, F32):
+            buf = torch.full((m, n + 40), 3.0, dtype=dtype, device="cuda")
+            for out in (buf[:, 16:16 + n], torch.empty(m, n, dtype=dtype, device="cuda")):
+                ops.gemm_nt_f8(x8, w8, sx.float(), sw.float(), out, **kw)
+                assert torch.equal(out.float(), want.float()), (list(kw), dtype)
+            assert (buf[:, :16] == 3.0).all() and (buf[:, 16 + n:] == 3.0).all()
+    ops.poll_status()
+
+
+@pytest.mark.parametrize("n", [328, 512])
+@pytest.mark.parametrize("m,code", [(333, c) for c in CODES] + [(20, c) for c in SMALL_CODES])
+def test_gemm_f8_activation_and_two_residuals(cuda_device, in_kernel, m, code, n):
+    """Sums as above are exact, so what is left is the activation (erf good to 5e-7, a few operations) and three additions."""
+    k = 400
+    x, w = whole(m, k, top=2, seed=m), whole(n, k, top=2, seed=n)
+    sx, sw = power(m, lo=-6, hi=-3, seed=1), power(n, lo=-2, hi=0, seed=2)
+    bias, r1, r2 = randn(n, seed=3).to(F16), randn(m, n, seed=4).to(F16), randn(m, n, seed=5).to(F16)
+    t = (x.double() @ w.double().t()) * sx[:, None] * sw + bias.double()
+    in_kernel(code)
+    out = torch.empty(m, n, dtype=F16, device="cuda")
+    ops.gemm_nt_f8(x.float().to(E4M3), w.float().to(E4M3), sx.float(), sw.float(), out, bias=bias, act="gelu", res1=r1, res2=r2)
+    mag = t.abs() + r1.double().abs() + r2.double().abs()
+    assert_fp16_close(out, gelu(t) + r1.double() + r2.double(), mag * 2.0 ** -20)
+    ops.poll_status()
 
 
 # ---- residuals of other shapes and strides -----------------------------------------------------------
