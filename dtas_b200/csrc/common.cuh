@@ -171,7 +171,7 @@ int launch_add_rms_norm(const void* x, const void* res, const void* weight, void
                         int64_t m, int64_t n_cols, float eps, int in_dtype, int out_dtype, const DeviceCtx* ctx, cudaStream_t st);
 int launch_quantize(const void* x, void* q, float* scale, int64_t m, int64_t n_cols, int in_dtype, int out_dtype,
                     const DeviceCtx* ctx, cudaStream_t st);
-void gemv_w4_variant_name(int64_t m, int64_t n, int64_t k, char* buf, int len);
+void gemv_w4_variant_name(int64_t m, int64_t n, int64_t k, const DeviceCtx* ctx, int device, char* buf, int len);
 void row_quant_variant_name(const char* op, int64_t m, int64_t n_cols, char* buf, int len);
 
 int launch_gemv_w4(const void* x, const float* x_scale, const void* w, const void* w_scale, const void* w_zero,

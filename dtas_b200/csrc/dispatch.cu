@@ -460,7 +460,7 @@ int dtas_variant_of(const char* op, int64_t m, int64_t n, int64_t k, int device,
     case 6: gemv_variant_name(n, k, ctx, buf, buf_len); break;
     case 7: gemm_variant_name(m, n, k, ctx, buf, buf_len); break;
     case 8: case 9: row_quant_variant_name(op, m, n, buf, buf_len); break;
-    case 10: gemv_w4_variant_name(m, n, k, buf, buf_len); break;
+    case 10: gemv_w4_variant_name(m, n, k, ctx, device, buf, buf_len); break;
     default: gemm_f8_variant_name(m, n, k, ctx, buf, buf_len); break;
   }
   return DTAS_OK;

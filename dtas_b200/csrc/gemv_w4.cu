@@ -754,13 +754,16 @@ struct W4Plan {
   int64_t smem;
 };
 
-// Clusters of c CTAs that the device holds at once: they do not pack every SM of its GPCs.  (B200: as the driver answers for
-// one CTA per SM; without a device the figures of one are assumed.)
-inline int w4_clusters(int c, int sm_count, const int* max_clusters) {
+// Clusters of c CTAs that the device holds at once: they do not pack every SM of its GPCs.  As the driver answers for one CTA
+// per SM (any instantiation: one fills an SM); before the first launch on a device the figures of a B200 are assumed.
+constexpr int kMaxDevices = 64;
+std::atomic<int> w4_max_clusters[kMaxDevices][3];      // of 2, 4 and 8 CTAs; 0: not asked yet
+inline int w4_clusters(int c, int sm_count, int device) {
   if (c == 1) return sm_count;
   const int slot = c == 2 ? 0 : (c == 4 ? 1 : 2);
   static const int assumed[3] = {74, 33, 15};
-  return max_clusters != nullptr && max_clusters[slot] > 0 ? max_clusters[slot] : assumed[slot];
+  const int n = device >= 0 && device < kMaxDevices ? w4_max_clusters[device][slot].load(std::memory_order_relaxed) : 0;
+  return n > 0 ? n : assumed[slot];
 }
 
 // A CTA takes a whole row's K where m rows of x fit beside its rings, else as many CTAs as it takes for a part of them to
@@ -769,12 +772,12 @@ inline int w4_clusters(int c, int sm_count, const int* max_clusters) {
 // sixteen rows, [4096, 11008], 21 us in four batches).  Items of 256 k, two to a ring, where there is room for them; else
 // of 128 k, two to four.  Deeper rings only let the first items of some warps queue behind later items of others
 // ([12288, 4096], one token: 10.7 us with two items of 256 k, 13.7 with three).
-inline W4Plan w4_plan(int64_t m, int64_t n, int64_t k, int64_t group, bool zero, int sm_count, const int* max_clusters) {
+inline W4Plan w4_plan(int64_t m, int64_t n, int64_t k, int64_t group, bool zero, int sm_count, int device) {
   W4Plan p{};
   const int64_t groups = k / group, cols = m <= 8 ? 8 : 16;
   p.sh.n_tiles = (int)((n + kRows - 1) / kRows);
   for (int c = 1; c <= kMaxCluster; c *= 2) {
-    const int most = w4_clusters(c, sm_count, max_clusters), n_clusters = p.sh.n_tiles < most ? p.sh.n_tiles : most;
+    const int most = w4_clusters(c, sm_count, device), n_clusters = p.sh.n_tiles < most ? p.sh.n_tiles : most;
     const int band = (p.sh.n_tiles + n_clusters - 1) / n_clusters;
     const int64_t xrows = (m + c - 1) / c;
     for (int ik = m <= 8 && c == 1 ? 256 : 128; ik >= 128; ik /= 2) {
@@ -821,14 +824,14 @@ EncodeTiledFn w4_encode_fn() {
 
 template <int IK, int NT, int GS, bool ZERO>
 int launch_one(const W4Args& a, int x_dtype, const DeviceCtx* ctx, cudaStream_t st) {
-  static std::atomic<bool> ready[64];
-  static int max_clusters[64][3];
+  static std::atomic<bool> ready[kMaxDevices];
   int dev = 0;
   DTAS_CUDA(cudaGetDevice(&dev));
-  if (dev >= 64) DTAS_FAIL(DTAS_EINVAL, "gemv_w4: device ordinal %d out of range", dev);
+  if (dev >= kMaxDevices) DTAS_FAIL(DTAS_EINVAL, "gemv_w4: device ordinal %d out of range", dev);
   if (!ready[dev].load(std::memory_order_acquire)) {
     DTAS_CUDA(cudaFuncSetAttribute((gemv_w4_kernel<IK, NT, GS, ZERO>), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMax));
     for (int i = 0; i < 3; ++i) {
+      if (w4_max_clusters[dev][i].load(std::memory_order_relaxed) != 0) continue;
       cudaLaunchConfig_t cfg = {};
       cudaLaunchAttribute attr;
       cfg.gridDim = dim3((unsigned)(2 << i));
@@ -844,11 +847,11 @@ int launch_one(const W4Args& a, int x_dtype, const DeviceCtx* ctx, cudaStream_t 
         (void)cudaGetLastError();
         n = 0;
       }
-      max_clusters[dev][i] = n;
+      w4_max_clusters[dev][i].store(n, std::memory_order_relaxed);
     }
     ready[dev].store(true, std::memory_order_release);
   }
-  const W4Plan p = w4_plan(a.m, a.n, a.k, a.group, ZERO, ctx->sm_count, max_clusters[dev]);
+  const W4Plan p = w4_plan(a.m, a.n, a.k, a.group, ZERO, ctx->sm_count, dev);
   if (p.cluster == 0 || p.item_k != IK) DTAS_FAIL(DTAS_EUNSUPPORTED, "gemv_w4: no plan");      // the caller has asked
   // q as bytes [n, k / 2], boxes of 32 rows by IK / 2 bytes; what lies outside arrives as zeros
   const EncodeTiledFn encode = w4_encode_fn();
@@ -905,7 +908,7 @@ int launch_x(const W4Args& a, int x_dtype, const DeviceCtx* ctx, cudaStream_t st
   const bool fast = w4_fast_shape(a.k, a.group) && aligned16(a.q) && aligned16(a.x) && aligned16(a.w_scale) && aligned16(a.zero);
   if (!fast) return launch_scalar<XT>(a, st);
   // whether a plan exists, and its items, do not depend on how many clusters the device holds
-  const W4Plan p = w4_plan(a.m, a.n, a.k, a.group, a.zero != nullptr, ctx->sm_count, nullptr);
+  const W4Plan p = w4_plan(a.m, a.n, a.k, a.group, a.zero != nullptr, ctx->sm_count, -1);
   if (p.cluster == 0) return launch_scalar<XT>(a, st);
   if (a.group == 32) return launch_zero<1>(a, p.item_k, x_dtype, ctx, st);
   if (a.group == 64) return launch_zero<2>(a, p.item_k, x_dtype, ctx, st);
@@ -915,8 +918,8 @@ int launch_x(const W4Args& a, int x_dtype, const DeviceCtx* ctx, cudaStream_t st
 }  // namespace
 
 // Named for groups of 128 without zero points.
-void gemv_w4_variant_name(int64_t m, int64_t n, int64_t k, char* buf, int len) {
-  const W4Plan p = w4_plan(m, n, k, 128, false, 148, nullptr);
+void gemv_w4_variant_name(int64_t m, int64_t n, int64_t k, const DeviceCtx* ctx, int device, char* buf, int len) {
+  const W4Plan p = w4_plan(m, n, k, 128, false, ctx->sm_count, device);
   if (k % kStep != 0 || p.cluster == 0) snprintf(buf, len, "gemv_w4_scalar_warp_per_element");
   else snprintf(buf, len, "gemv_w4_mma_m%d_k%d_s%d_cluster%d", m <= 8 ? 8 : 16, p.item_k, p.sh.stages, p.cluster);
 }
