@@ -285,7 +285,8 @@ int dtas_gemm_nt_fused(const void* x, const void* w, const void* bias, const voi
   // Behind a large GEMM the residual rows cost less as one streaming pass over Y (every thread of the
   // GEMM epilogue owns a row, so its residual loads touch 32 rows per instruction): measured at
   // m = 4096, N = K = 2560, two residuals: 76 us in the epilogue, 70 us as GEMM + two adds.
-  const bool own_pass = res1 != nullptr && !epi.out_f32 && m >= kResidualPassMinRows && ldy == n && ldr == n;
+  // A residual that lies where Y does is gone by then, so it stays in the epilogue, which reads before it stores.
+  const bool own_pass = res1 != nullptr && !epi.out_f32 && m >= kResidualPassMinRows && ldy == n && ldr == n && res1 != y && res2 != y;
   if (!own_pass) {
     epi.res1 = static_cast<const __half*>(res1);
     epi.res2 = static_cast<const __half*>(res2);

@@ -110,7 +110,8 @@ int dtas_gemm_nt(const void* x, const void* w, const void* bias, void* y,
  * fp16 value widened to fp32.  bias [n], res1 and res2 [m, n] (row stride ldr elements; [n] for
  * the GEMV) are fp16 and optional (NULL); res2 needs res1.  act is DTAS_ACT_NONE or
  * DTAS_ACT_GELU = t * (0.5 + 0.5 * erf(t / sqrt(2))), the erf form of the reference's workload.
- * The reference rounds every intermediate to fp16; results agree within the GEMM tolerance.   */
+ * The reference rounds every intermediate to fp16; results agree within the GEMM tolerance.
+ * A residual may be y itself (the same address and row stride): it is read before it is overwritten.  */
 #define DTAS_ACT_NONE 0
 #define DTAS_ACT_GELU 1
 int dtas_gemm_nt_fused(const void* x, const void* w, const void* bias, const void* res1, const void* res2,

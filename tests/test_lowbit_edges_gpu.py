@@ -226,6 +226,38 @@ def test_gemm_f8_activation_and_two_residuals(cuda_device, in_kernel, m, code, n
     ops.poll_status()
 
 
+@pytest.mark.parametrize("m", [300, 2100])
+def test_gemm_into_its_own_residual(cuda_device, m):
+    n, k = 264, 128
+    x, w, r, r2 = (whole(*s, top=2, seed=i).to(F16) for i, s in enumerate(((m, k), (n, k), (m, n), (m, n))))
+    want = x.double() @ w.double().t() + r.double() + r2.double()
+    for first in (True, False):
+        out = r.clone()
+        ops.gemm_nt(x, w, out, res1=out if first else r2, res2=r2 if first else out)
+        assert torch.equal(out.double(), want)
+
+
+@pytest.mark.parametrize("n", [328, 333])
+@pytest.mark.parametrize("m,code", [(m, c) for m in (200, 333) for c in CODES] + [(m, c) for m in (1, 20, 50) for c in SMALL_CODES] + [(2100, (0, 0))])
+def test_low_bit_products_into_their_own_residual(cuda_device, in_kernel, m, code, n):
+    """The residual stream as both an operand and the result: every element is read before it is stored."""
+    k = 400
+    x, w = whole(m, k, top=2, seed=m), whole(n, k, top=2, seed=n)
+    r, r2 = whole(m, n, top=64, seed=4).to(F16), whole(m, n, top=64, seed=5).to(F16)
+    one = torch.ones(max(m, n), device="cuda")
+    in_kernel(code)
+    want = x.double() @ w.double().t() + r.double() + r2.double()
+    for first in (True, False):
+        out = r.clone()
+        ops.gemm_nt_f8(x.float().to(E4M3), w.float().to(E4M3), one[:m], one[:n], out, res1=out if first else r2, res2=r2 if first else out)
+        assert torch.equal(out.double(), want)
+    if m <= 16:
+        codes = (w + 8).to(torch.uint8)
+        out = r.clone()
+        ops.gemv_w4(x.to(F16), weights.pack_w4(codes), torch.ones(n, 1, dtype=F16, device="cuda"), out, res1=out, res2=r2)
+        assert torch.equal(out.double(), want)
+
+
 # ---- residuals of other shapes and strides -----------------------------------------------------------
 def test_residuals_of_other_shapes_are_refused(cuda_device):
     m, n, k = 12, 24, 64
