@@ -344,7 +344,7 @@ def add_rms_norm(x, res, weight, out, res_out=None, scale=None, eps=1e-6):
 
 
 def _check_quantize(x, out, scale):
-    _check("quantize", x, out, scale)
+    _check("quantize", *[t for t in (x, out, scale) if t is not None])
     _same_shape("quantize", x, out)
     if x.dtype not in _IN_CODE:
         raise _abi.DtasError(_abi.EUNSUPPORTED, f"quantize: x must be fp16 or fp32, got {x.dtype}")
@@ -360,7 +360,7 @@ def quantize(x, out, scale):
     dev, shape, dtype = x.get_device(), x.shape, x.dtype
     code = _LOW_CODE.get(out.dtype)
     if (dev < 0 or code is None or dtype not in _IN_CODE or len(shape) != 2 or out.shape != shape or out.get_device() != dev
-            or scale.dtype != torch.float32 or scale.numel() != shape[0] or scale.get_device() != dev
+            or scale is None or scale.dtype != torch.float32 or scale.numel() != shape[0] or scale.get_device() != dev
             or not (x.is_contiguous() and out.is_contiguous() and scale.is_contiguous())):
         _check_quantize(x, out, scale)
     status = (_L or _lib()).dtas_quantize(x.data_ptr(), out.data_ptr(), scale.data_ptr(), shape[-2], shape[-1], _IN_CODE[dtype],

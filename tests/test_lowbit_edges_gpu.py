@@ -274,6 +274,14 @@ def test_residuals_of_other_shapes_are_refused(cuda_device):
     assert (out == 3.0).all()
 
 
+def test_rows_without_a_scale_are_refused(cuda_device):
+    x, q = torch.zeros(2, 8, dtype=F16, device="cuda"), torch.zeros(2, 8, dtype=I8, device="cuda")
+    for call in (lambda: ops.quantize(x, q, None), lambda: ops.add_rms_norm(x, None, x[0], q)):
+        with pytest.raises(_abi.DtasError) as e:
+            call()
+        assert e.value.code == _abi.EINVAL
+
+
 # ---- 4-bit products: what is not finite --------------------------------------------------------------
 def w4_operands(m, n, k, group, zero, seed=0):
     """x, codes [N, K], packed codes, scales, zero points or None."""
