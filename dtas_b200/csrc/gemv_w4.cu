@@ -20,10 +20,10 @@
 // the pairs that the masks cut out of a word are (k, k + 4), so x is paired the same way.  A group's sums enter the
 // row's fp32 sum with one multiply by the group's scale; x in 8 bits is widened to fp16, which holds it exactly.
 //
-// Measured, HBM 6.57 TB/s: one row by [22016, 4096] in groups of 32, bias and GELU 15.8 us (3.2 TB/s; its bytes take 7.7), by
-// [4096, 4096] 5.9 us; sixteen rows by [4096, 11008] with zero points 17.5 us; four e4m3 rows by [50280, 2560] in groups of
-// 64 17.8 us (3.9 TB/s).  Neither loads nor a pipe are at their limit: fetching the long unrolled body, unpacking and
-// the scale per group come on top of the stream.
+// Measured, HBM 6.57 TB/s: one row by [22016, 4096] in groups of 32, bias and GELU 15.7 us (3.2 TB/s; its bytes take 7.7), by
+// [4096, 4096] 5.8 us; sixteen rows by [4096, 11008] with zero points 19.0 us; four e4m3 or int8 rows by [50280, 2560] in groups of
+// 64 17.6 us (3.9 TB/s).  Neither loads nor a pipe are at their limit, and with the codes in L2 it takes as long: three warps a
+// scheduler take half of the issue slots between the preparation of x and the exchange of the sums.
 #include <cuda.h>
 #include <cuda_fp8.h>
 

@@ -21,8 +21,8 @@
 // every operand (EDGE): chunks are cut where the flat index is a multiple of eight, loads take whole vectors, and of the
 // results only the first and the last chunk of a row, which it shares with its neighbours, go element by element.
 // Where the rows fill the device several times over, CTAs stay and take rows in turn (row_quant_stream_kernel).
-// Measured (HBM 6.57 TB/s): add_rms_norm fp16 to e4m3 [8192, 4096] 39.8 us, 5.9 TB/s; fp32 [4096, 4096] 33.3 us, 6.5 TB/s;
-// [1, 4096] 1.9 us; quantize to e4m3 [2048, 11008] 14.9 us, 4.5 TB/s; [8192, 4096] 17.6 us, 5.7 TB/s.
+// Measured (HBM 6.57 TB/s): add_rms_norm fp16 to e4m3 [8192, 4096] 39.1 us, 6.0 TB/s; fp32 [4096, 4096] 34.5 us, 6.3 TB/s;
+// [1, 4096] 1.8 us; quantize to e4m3 [2048, 11008] 15.0 us, 4.5 TB/s; [8192, 4096] 17.6 us, 5.7 TB/s.
 #include <cuda_fp8.h>
 
 #include <atomic>

@@ -218,7 +218,8 @@ def gemm_nt(x, w, out, bias=None, res1=None, res2=None, act=None):
     are optional: the fused forms of the reference's model workloads.
 
     `out` may be a column slab of a wider row-major buffer (last-dim stride 1, any row
-    stride >= N): a column-sharded rank writes its part of the full output in place.
+    stride >= N): a column-sharded rank writes its part of the full output in place.  So may res1 and res2,
+    with one row stride; either may be `out` itself.
     """
     dev_t = x.device
     if dev_t.type != "cuda":
@@ -397,7 +398,8 @@ def gemv_w4(x, w, w_scale, out, w_zero=None, x_scale=None, bias=None, res1=None,
     `w` is uint8 [N, K / 2], two codes to a byte, the even k in the low half; `w_scale` fp16 [N, K / G] says
     what G is; `w_zero` uint8 of the same shape, 8 everywhere when None (dtas_b200.weights.quantize_w4
     makes all three).  x is fp16, or int8 / float8_e4m3fn with x_scale fp32 [m], as add_rms_norm and
-    quantize write them.  out is fp16 or fp32 (the fp16 result widened); the tail is that of gemv."""
+    quantize write them.  out is fp16 or fp32 (the fp16 result widened); the tail is that of gemv, and res1 or res2
+    may be `out` itself."""
     dev, xs, os, gs, dtype = x.get_device(), x.shape, out.shape, w_scale.shape, x.dtype
     code = _W4_IN.get(dtype)
     if (dev < 0 or code is None or len(xs) != 2 or len(os) != 2 or len(gs) != 2 or xs[0] != os[0] or os[1] != gs[0]
@@ -452,7 +454,8 @@ def _check_gemm_nt_f8(x, w, x_scale, w_scale, out, bias, res1, res2, act):
 def gemm_nt_f8(x, w, x_scale, w_scale, out, bias=None, res1=None, res2=None, act=None):
     """out[m, N] = act(x_scale[m] * w_scale[N] * (x[m, K] @ w[N, K]^T) + bias[N]) + res1 + res2 of float8_e4m3fn
     operands with fp32 scales per row of x and per row of w (as quantize writes them); fp32 accumulation,
-    fp16 or fp32 `out`.  The tail, and an `out` that is a column slab of a wider buffer, are those of gemm_nt."""
+    fp16 or fp32 `out`.  The tail, residuals and an `out` that are column slabs of wider buffers, and a residual that is
+    `out` itself, are those of gemm_nt."""
     dev, xs, ws, os, ldr = x.get_device(), x.shape, w.shape, out.shape, 0
     f8 = torch.float8_e4m3fn
     if (dev < 0 or len(xs) != 2 or len(ws) != 2 or len(os) != 2 or xs[1] != ws[1] or os != (xs[0], ws[0])

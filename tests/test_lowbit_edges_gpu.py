@@ -235,6 +235,9 @@ def test_gemm_into_its_own_residual(cuda_device, m):
         out = r.clone()
         ops.gemm_nt(x, w, out, res1=out if first else r2, res2=r2 if first else out)
         assert torch.equal(out.double(), want)
+        row, other = r[:1].clone(), r2[:1]
+        ops.gemv(x[:1], w, row, res1=row if first else other, res2=other if first else row)
+        assert torch.equal(row.double(), want[:1])
 
 
 @pytest.mark.parametrize("n", [328, 333])
