@@ -406,3 +406,115 @@ def test_calls_keep_stream_order(cuda_device, m, h, f):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(chain.outs, want))
     ops.poll_status()
+
+
+# ---- the calls' other forms: sizes, shapes, threads ----------------------------------------------------
+@pytest.mark.parametrize("h", [16384, 16383])
+def test_rows_beyond_32_bit_offsets(cuda_device, h):
+    """More than 2^31 elements: rows on both sides of the border are those that a call of their own gives."""
+    m = 2 ** 31 // h + 40
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.empty(m, h, dtype=F16, device="cuda").normal_(generator=g)
+    weight = (1 + randn(h, seed=3, scale=0.1)).to(F16)
+    rows = torch.tensor([0, 1, m // 2, m - 41, m - 40, m - 39, m - 2, m - 1], device="cuda")
+    some = x[rows].clone()
+    q, scale = torch.empty(m, h, dtype=I8, device="cuda"), torch.empty(m, device="cuda")
+    q1, s1 = torch.empty(len(rows), h, dtype=I8, device="cuda"), torch.empty(len(rows), device="cuda")
+    ops.quantize(x, q, scale)
+    ops.quantize(some, q1, s1)
+    assert torch.equal(q[rows], q1) and torch.equal(scale[rows], s1)
+    twice = some.float() * 2
+    ops.add_rms_norm(some, some, weight, q1, scale=s1)
+    ops.add_rms_norm(x, x, weight, q, res_out=x, scale=scale)
+    assert torch.equal(q[rows], q1) and ((scale[rows] - s1).abs() <= s1 * 2.0 ** -18).all()
+    assert torch.equal(x[rows].float(), twice)
+
+
+def test_products_beyond_32_bit_offsets(cuda_device):
+    """Weights, results and residuals of more than 2^31 elements."""
+    def eight(t):
+        return t.float().to(E4M3)
+
+    m, n, k = 270000, 8192, 64                                    # y and the residual, which is y
+    x, w = whole(m, k, top=2, seed=1), whole(n, k, top=2, seed=2)
+    y = torch.ones(m, n, dtype=F16, device="cuda")
+    ops.gemm_nt_f8(eight(x), eight(w), torch.ones(m, device="cuda"), torch.ones(n, device="cuda"), y, res1=y)
+    rows = torch.tensor([0, 2 ** 31 // n - 1, 2 ** 31 // n, m - 1], device="cuda")
+    assert torch.equal(y[rows].double(), x[rows].double() @ w.double().t() + 1)
+    del y
+    m, n, k = 3, 262145, 8208                                     # w, for both products
+    x, w = whole(m, k, top=2, seed=1), torch.zeros(n, k, dtype=torch.uint8, device="cuda")
+    rows = torch.tensor([0, 2 ** 31 // k, 2 ** 31 // k + 1, n - 1], device="cuda")
+    w[rows] = (whole(4, k, top=7, seed=3) + 8).to(torch.uint8)
+    y = torch.empty(m, n, dtype=F16, device="cuda")
+    ops.gemm_nt_f8(eight(x), w.to(E4M3), torch.ones(m, device="cuda"), torch.ones(n, device="cuda"), y)
+    assert torch.equal(y[:, rows].float(), (x.double() @ w[rows].double().t()).float().to(F16).float())
+    m, n, k, group = 9, 1048577, 4096, 32                         # codes, and 2^27 scales
+    x = whole(m, k, top=2, seed=1)
+    codes = torch.full((n, k // 2), 0x88, dtype=torch.uint8, device="cuda")
+    rows = torch.tensor([0, 2 ** 20 - 1, 2 ** 20, n - 1], device="cuda")
+    some = whole(4, k, top=7, seed=3) + 8
+    codes[rows] = weights.pack_w4(some.to(torch.uint8))
+    y = torch.empty(m, n, dtype=F16, device="cuda")
+    ops.gemv_w4(x.to(F16), codes, torch.ones(n, k // group, dtype=F16, device="cuda"), y)
+    held = torch.stack((codes[rows] & 15, codes[rows] >> 4), -1).view(4, k).double() - 8      # the last two rows are one
+    assert torch.equal(y[:, rows].float(), (x.double() @ held.t()).float().to(F16).float())
+    y[:, rows] = 0
+    assert (y == 0).all()
+    ops.poll_status()
+
+
+def test_operands_with_a_leading_unit_dimension(cuda_device):
+    """[1, m, H] beside [m, H], in every operand that has rows."""
+    m, n, k = 5, 48, 64
+    lead = lambda t: t.unsqueeze(0)  # noqa: E731
+    x, res, weight = randn(m, k, seed=1).to(F16), randn(m, k, seed=2).to(F16), (1 + randn(k, seed=3, scale=0.1)).to(F16)
+    got = [[torch.empty(m, k, dtype=E4M3, device="cuda"), torch.empty(m, device="cuda"), torch.empty_like(x)] for _ in range(2)]
+    ops.add_rms_norm(x, res, weight, got[0][0], res_out=got[0][2], scale=got[0][1])
+    ops.add_rms_norm(lead(x), res, lead(lead(weight)), lead(got[1][0]), res_out=lead(got[1][2]), scale=lead(got[1][1]))
+    assert all(torch.equal(a.float(), b.float()) for a, b in zip(*got))
+    rows, scale, _ = got[0]
+    q, s = torch.empty_like(rows), torch.empty_like(scale)
+    ops.quantize(lead(x), lead(q), s)
+    ops.quantize(x, rows, scale)
+    assert torch.equal(q.float(), rows.float()) and torch.equal(s, scale)
+    r, bias = randn(m, n, seed=4).to(F16), randn(n, seed=5).to(F16)
+    w8, ws = torch.empty(n, k, dtype=E4M3, device="cuda"), torch.empty(n, device="cuda")
+    ops.quantize(randn(n, k, seed=6).to(F16), w8, ws)
+    codes, scales, zeros = weights.quantize_w4(randn(n, k, seed=7), 32, True)
+    wide = torch.zeros(1, m, 3 * n, dtype=F16, device="cuda")
+    for call in (lambda a, b, o: ops.gemm_nt_f8(a, w8, scale, ws, o, bias=bias, res1=b, act="gelu"),
+                 lambda a, b, o: ops.gemv_w4(a, codes, scales, o, w_zero=zeros, x_scale=scale, bias=bias, res1=b, act="gelu")):
+        want = call(rows, r, torch.empty(m, n, dtype=F16, device="cuda"))
+        assert torch.equal(call(lead(rows), lead(r), torch.empty(1, m, n, dtype=F16, device="cuda"))[0], want)
+        assert torch.equal(call(lead(rows), r, torch.empty(m, n, dtype=F16, device="cuda")), want)
+    slab = wide[:, :, n:2 * n]
+    ops.gemm_nt_f8(lead(rows), w8, scale, ws, slab, bias=bias, res1=lead(r), act="gelu")
+    assert torch.equal(slab[0], ops.gemm_nt_f8(rows, w8, scale, ws, torch.empty(m, n, dtype=F16, device="cuda"), bias=bias, res1=r, act="gelu"))
+    assert (wide[:, :, :n] == 0).all() and (wide[:, :, 2 * n:] == 0).all()
+
+
+def test_calls_from_several_threads(cuda_device):
+    """Host threads with streams of their own, all calls at once: every one gets what it gets alone."""
+    import threading
+    chains = [Chain(m, 1024, 4096) for m in (1, 3, 8, 16)]
+    want = [c.run(sync=True) for c in chains]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(10):
+                got = chains[i].run(sync=False)
+                stream.synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    failed.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(chains))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    ops.poll_status()
